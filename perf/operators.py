@@ -216,9 +216,12 @@ def _attention_plain(s):
     ds = p * (dp - (do * out).sum(3, keepdim=True))
     dq = (ds @ ke) * scale
     dk = ((ds.transpose(2, 3) @ q) * scale).reshape(b, hk, group, sk, d).sum(2)
-    per_head = ds.sum(0, dtype=torch.float64).reshape(h, sq * sk)
-    member = (bucket.reshape(-1, 1) == torch.arange(c["buckets"], device=q.device)).double()
-    table = per_head @ member
+    # the table's gradient: every relative position is a diagonal; rows reversed and shifted make it a column
+    skew = torch.nn.functional.pad(ds.sum(0, dtype=torch.float64).flip(1), (0, sq)).reshape(h, -1)[:, :sq * (sk + sq - 1)]
+    of_rel = skew.reshape(h, sq, sk + sq - 1).sum(1)
+    rels = torch.arange(-(sk - 1), sq, device=q.device)
+    member = _buckets(rels, c["buckets"], c["distance"], c["both"])[:, None] == torch.arange(c["buckets"], device=q.device)
+    table = of_rel @ member.double()
     return {"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv, "dtable": table.t().float().contiguous()}
 
 
