@@ -28,6 +28,28 @@ struct ProfScope {
     ~ProfScope() { if (slot != -1) prof_close(slot); }
 };
 
+// Around the launches of an entry point: the library's device is made the thread's current one and the caller's is put back
+// behind it (a caller with several GPUs may have another one selected).  rc is BH_EINVAL while the library's stream is being
+// captured into a graph: device memory of the cache would be handed to other calls while a graph still writes to it.
+struct CallGuard {
+    int rc = BH_OK, previous = -1;
+    explicit CallGuard(const char* fn);
+    ~CallGuard();
+    CallGuard(const CallGuard&) = delete;
+};
+#define BH_CALL_GUARD()                       \
+    ::bh::CallGuard call_guard__(__func__);   \
+    if (call_guard__.rc) return call_guard__.rc
+
+// device memory for the kernels of one call; given back to the cache when the call returns (reuse is ordered by the stream)
+struct Scratch {
+    void* p = nullptr;
+    bool get(size_t nbytes) { return (p = bh_malloc(nbytes)) != nullptr; }
+    Scratch() = default;
+    Scratch(const Scratch&) = delete;
+    ~Scratch() { if (p) bh_free(p); }
+};
+
 #define BH_REQUIRE_INIT()                                   \
     do {                                                    \
         if (!::bh::ready()) {                               \

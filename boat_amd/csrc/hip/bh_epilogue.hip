@@ -1,0 +1,510 @@
+// bh_epilogue.hip - a matrix product whose stores finish the layer: C = act(op(A).op(B) + bias) + residual.
+//
+// A dense layer of a transformer is z = x.W + b, y = act(z), and often h = y + residual (src/layers/dense.c:135-188 and the
+// elementwise passes behind it).  Each pass behind the product reads and writes the whole [rows, features] matrix; here the
+// accumulators go through bias, activation and residual in registers, and what the backward pass needs (z, or act(z) for the
+// activations whose derivative is a function of it) is stored beside the result.
+//
+// The products run on the bf16 matrix cores from operands split into three bf16 each (bh_split.h): fp32 sums at six bf16
+// instructions per product, 2.7 times the rate of the fp32 matrix instruction.
+#include "bh_split.h"
+
+#include <math.h>
+
+namespace bh {
+
+struct EpiArgs {
+    const float* a; const float* b;
+    int64_t m, n, k, lda, ldb;
+    float* c; int64_t ldc;
+    const float* bias;                       // [n] or NULL
+    float* saved; int64_t lds;               // [m, n] or NULL
+    const float* residual; int64_t ldr;      // [m, n] or NULL; may be c itself
+    int act;
+    int tiles_m, tiles_n;
+    int splits;                              // > 1: partial sums go to `partial` [split][m][n], epilogue_fold_kernel finishes
+    int64_t k_per_split;                     // multiple of 16
+    float* partial;
+};
+
+__device__ __forceinline__ float act_value(int act, float z) {
+    switch (act) {
+        case BH_ACT_RELU: return z > 0.f || z != z ? z : 0.f;
+        case BH_ACT_SIGMOID: return 1.f / (1.f + expf(-z));
+        case BH_ACT_TANH: return tanhf(z);
+        case BH_ACT_GELU: return z * (0.5f * (1.f + erff(z * 0.70710678118654752440f)));
+    }
+    return z;
+}
+// what bh_activation_backward reads: the input of ReLU and GELU, the output of sigmoid and tanh
+__device__ __forceinline__ bool saves_output(int act) { return act == BH_ACT_SIGMOID || act == BH_ACT_TANH; }
+
+__device__ __forceinline__ bool finite_f32(float v) { return fabsf(v) <= 3.402823466e38f; }
+
+// one element of the product in plain fp32 arithmetic: for sums the split could not carry (infinities, NaN)
+template <bool A_KC, bool B_KC>
+__device__ __forceinline__ float plain_element(const EpiArgs& g, int64_t row, int64_t col, int64_t k0, int64_t k1) {
+    float s = 0.f;
+    for (int64_t k = k0; k < k1; k++) {
+        const float x = A_KC ? g.a[row * g.lda + k] : g.a[k * g.lda + row];
+        const float y = B_KC ? g.b[col * g.ldb + k] : g.b[k * g.ldb + col];
+        s = fmaf(x, y, s);
+    }
+    return s;
+}
+
+__device__ __forceinline__ void finish_element(const EpiArgs& g, int64_t row, int64_t col, float sum) {
+    float z = sum + (g.bias ? g.bias[col] : 0.f);
+    float y = act_value(g.act, z);
+    if (g.saved) g.saved[row * g.lds + col] = saves_output(g.act) ? y : z;
+    if (g.residual) y += g.residual[row * g.ldr + col];
+    g.c[row * g.ldc + col] = y;
+}
+
+// workgroup number -> output tile: neighbours in launch order go to different XCDs, so each XCD gets a contiguous run of
+// tiles (its own L2), walked in groups of 8 tile rows
+__device__ __forceinline__ void tile_of(int pid, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int total = tiles_m * tiles_n;
+    if (total % kNumXcd == 0) pid = (pid % kNumXcd) * (total / kNumXcd) + pid / kNumXcd;
+    constexpr int kGroup = 8;
+    const int per = kGroup * tiles_n, first = pid / per * kGroup;
+    const int rows = min(tiles_m - first, kGroup);
+    tm = first + pid % per % rows;
+    tn = pid % per / rows;
+}
+
+// ---------------------------------------------------------------------------------------------------- finishing a tile
+// A wavefront's finished 32 x (32*TN) block of sums goes through LDS (rows padded by 8 floats), so that the rest runs over
+// whole rows: 16-byte loads and stores, one copy of the activation's code, and the rare recomputation can index its element.
+template <int TN> struct EpiBlock {
+    static constexpr int LD = 32 * TN + 8;       // floats
+    static constexpr int BYTES = 32 * LD * (int)sizeof(float);
+};
+
+template <int TN, bool A_KC, bool B_KC>
+__device__ __forceinline__ void finish_block(const EpiArgs& g, const f32x16 (&acc)[TN], float* lds, int64_t row0, int64_t col0, int lane,
+                                             bool vec) {
+    constexpr int LD = EpiBlock<TN>::LD;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) lds[acc_row(e, lane) * LD + 32 * j + (lane & 31)] = acc[j][e];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    constexpr int LANES = 8 * TN;                // lanes of a row, 4 columns each
+    const int64_t col = col0 + 4 * (lane % LANES);
+    const bool whole = vec && col + 4 <= g.n;
+    f32x4 bias = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+        if (g.bias && col + q < g.n) bias[q] = g.bias[col + q];
+#pragma unroll 2
+    for (int r = lane / LANES; r < 32; r += 64 / LANES) {
+        const int64_t row = row0 + r;
+        if (row >= g.m) break;
+        f32x4 z = *reinterpret_cast<const f32x4*>(lds + r * LD + 4 * (lane % LANES));
+        const float t = (z[0] - z[0]) + (z[1] - z[1]) + (z[2] - z[2]) + (z[3] - z[3]);
+        if (t != 0.f) {                          // NaN: some sum is not finite
+            for (int q = 0; q < 4; q++) {
+                const float v = lds[r * LD + 4 * (lane % LANES) + q];
+                const float w = finite_f32(v) || col + q >= g.n ? v : plain_element<A_KC, B_KC>(g, row, col + q, 0, g.k);
+                if (q == 0) z[0] = w; else if (q == 1) z[1] = w; else if (q == 2) z[2] = w; else z[3] = w;
+            }
+        }
+        z += bias;
+        f32x4 y;
+#pragma unroll
+        for (int q = 0; q < 4; q++) y[q] = act_value(g.act, z[q]);
+        const f32x4 keep = saves_output(g.act) ? y : z;
+        if (whole) {
+            if (g.saved) *reinterpret_cast<f32x4*>(g.saved + row * g.lds + col) = keep;
+            if (g.residual) y += *reinterpret_cast<const f32x4*>(g.residual + row * g.ldr + col);
+            *reinterpret_cast<f32x4*>(g.c + row * g.ldc + col) = y;
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (col + q >= g.n) break;
+                if (g.saved) g.saved[row * g.lds + col + q] = keep[q];
+                if (g.residual) y[q] += g.residual[row * g.ldr + col + q];
+                g.c[row * g.ldc + col + q] = y[q];
+            }
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+}
+
+// ---------------------------------------------------------------------------------------------------- tiles through LDS
+// One operand of R output rows, 16 of the contraction per stage.  LDS holds the three bf16 planes in fragment order: for each
+// half of the 16 (kg) R x 16 bytes, so a fragment is one ds_read_b128 at consecutive addresses.
+// KC: the contraction index is the fast one in memory (a thread takes 8 consecutive floats of one row, its neighbour the other
+// half: the padding keeps the two halves' writes in different banks); otherwise the output index is (a thread takes 8 floats
+// down one column).
+template <bool KC, int R, int NT>
+struct SplitOperand {
+    static constexpr int KG = 16 * R + 64;
+    static constexpr int PLANE = 2 * KG;
+    static constexpr int BYTES = kPlanes * PLANE;
+    static constexpr int PER = 2 * R / NT;                          // units (row, half of the 16) of a thread
+    static_assert(2 * R % NT == 0, "whole units per thread");
+
+    float reg[PER][8];
+
+    static __device__ __forceinline__ void unit(int tid, int i, int& row, int& kg) {
+        const int u = tid + i * NT;
+        if (KC) { row = u >> 1; kg = u & 1; } else { row = u % R; kg = u / R; }
+    }
+    // rows past the matrix are clamped (their products are not stored), the tail of the contraction is zero
+    __device__ __forceinline__ void load(const float* __restrict__ p, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int64_t k1,
+                                         bool vec, int tid) {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            int row, kg;
+            unit(tid, i, row, kg);
+            int64_t r = row0 + row;
+            if (r >= rows) r = rows - 1;
+            const int64_t k = k0 + 8 * kg;
+            if (k0 + 16 <= k1) {
+                if (KC) {
+                    const float* q = p + r * ld + k;
+                    if (vec) {
+                        const f32x4 x = *reinterpret_cast<const f32x4*>(q), y = *reinterpret_cast<const f32x4*>(q + 4);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) { reg[i][e] = x[e]; reg[i][4 + e] = y[e]; }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) reg[i][e] = q[e];
+                    }
+                } else {
+                    const float* q = p + k * ld + r;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) reg[i][e] = q[e * ld];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) reg[i][e] = k + e < k1 ? (KC ? p[r * ld + k + e] : p[(k + e) * ld + r]) : 0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char* lds, int tid) const {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            int row, kg;
+            unit(tid, i, row, kg);
+            u32x4 p[kPlanes];
+            split_eight(reg[i], p);
+#pragma unroll
+            for (int q = 0; q < kPlanes; q++) *reinterpret_cast<u32x4*>(lds + q * PLANE + kg * KG + row * 16) = p[q];
+        }
+    }
+    // rows 32*b .. 32*b + 31
+    static __device__ __forceinline__ void fragment(const char* lds, int b, int lane, u32x4 (&f)[kPlanes]) {
+#pragma unroll
+        for (int q = 0; q < kPlanes; q++)
+            f[q] = *reinterpret_cast<const u32x4*>(lds + q * PLANE + (lane >> 5) * KG + (32 * b + (lane & 31)) * 16);
+    }
+};
+
+template <int TM_, int TN_, int WM_, int WN_, int WGS_>
+struct SplitTile {
+    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, WGS = WGS_;   // WGS: wavefronts per SIMD the registers are held to
+    static constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, NT = 64 * WM * WN;
+};
+typedef SplitTile<2, 4, 4, 2, 2> Tile256;
+typedef SplitTile<2, 2, 2, 2, 2> Tile128;
+
+template <typename Cfg, bool A_KC, bool B_KC>
+struct TileLds {
+    static constexpr int STAGE = SplitOperand<A_KC, Cfg::BM, Cfg::NT>::BYTES + SplitOperand<B_KC, Cfg::BN, Cfg::NT>::BYTES;
+    static constexpr int EPI = Cfg::WM * Cfg::WN * EpiBlock<Cfg::TN>::BYTES;
+    static constexpr int BYTES = 2 * STAGE > EPI ? 2 * STAGE : EPI;
+};
+
+template <typename Cfg, bool A_KC, bool B_KC>
+__global__ __launch_bounds__(Cfg::NT, Cfg::WGS) void epilogue_tile_kernel(EpiArgs g, bool vec_a, bool vec_b, bool vec_c) {
+    constexpr int TM = Cfg::TM, TN = Cfg::TN;
+    using OpA = SplitOperand<A_KC, Cfg::BM, Cfg::NT>;
+    using OpB = SplitOperand<B_KC, Cfg::BN, Cfg::NT>;
+    constexpr int STAGE = TileLds<Cfg, A_KC, B_KC>::STAGE;
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
+    int tm, tn;
+    tile_of(blockIdx.x, g.tiles_m, g.tiles_n, tm, tn);
+    const int64_t m0 = (int64_t)tm * Cfg::BM, n0 = (int64_t)tn * Cfg::BN;
+    const int64_t kb = blockIdx.y * g.k_per_split, ke = min(g.k, kb + g.k_per_split);
+    const int steps = ke > kb ? (int)((ke - kb + 15) / 16) : 0;
+
+    f32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+
+    OpA oa;
+    OpB ob;
+    const auto fetch = [&](int s) {
+        oa.load(g.a, g.lda, m0, g.m, kb + 16 * s, ke, vec_a, tid);
+        ob.load(g.b, g.ldb, n0, g.n, kb + 16 * s, ke, vec_b, tid);
+    };
+    if (steps > 0) {
+        fetch(0);
+        oa.store(smem, tid);
+        ob.store(smem + OpA::BYTES, tid);
+        if (steps > 1) fetch(1);
+    }
+    __syncthreads();
+    for (int s = 0; s < steps; s++) {
+        const char* cur = smem + (s & 1) * STAGE;
+        char* next = smem + ((s & 1) ^ 1) * STAGE;
+        u32x4 fa[TM][kPlanes], fb[TN][kPlanes];
+#pragma unroll
+        for (int i = 0; i < TM; i++) OpA::fragment(cur, wm * TM + i, lane, fa[i]);
+#pragma unroll
+        for (int j = 0; j < TN; j++) OpB::fragment(cur + OpA::BYTES, wn * TN + j, lane, fb[j]);
+        if (s + 1 < steps) {                     // the other stage is free since the last barrier
+            oa.store(next, tid);
+            ob.store(next + OpA::BYTES, tid);
+        }
+        if (s + 2 < steps) fetch(s + 2);
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int j = 0; j < TN; j++) acc[i][j] = mfma_split(fa[i], fb[j], acc[i][j]);
+        __syncthreads();
+    }
+
+    const int64_t row0 = m0 + wm * 32 * TM, col0 = n0 + wn * 32 * TN;
+    if (g.splits > 1) {
+        float* part = g.partial + (int64_t)blockIdx.y * g.m * g.n;
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int64_t row = row0 + 32 * i + acc_row(e, lane);
+                if (row >= g.m) continue;
+#pragma unroll
+                for (int j = 0; j < TN; j++) {
+                    const int64_t col = col0 + 32 * j + (lane & 31);
+                    if (col < g.n) part[row * g.n + col] = acc[i][j][e];
+                }
+            }
+        return;
+    }
+    float* block = reinterpret_cast<float*>(smem + wave * EpiBlock<TN>::BYTES);
+#pragma unroll
+    for (int i = 0; i < TM; i++) finish_block<TN, A_KC, B_KC>(g, acc[i], block, row0 + 32 * i, col0, lane, vec_c);
+}
+
+// the splits' partial sums, added in order, through the epilogue
+template <bool A_KC, bool B_KC>
+__global__ __launch_bounds__(256) void epilogue_fold_kernel(EpiArgs g) {
+    const int64_t total = g.m * g.n;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        float sum = 0.f;
+        for (int s = 0; s < g.splits; s++) sum += g.partial[s * total + i];
+        const int64_t row = i / g.n, col = i - row * g.n;
+        if (!finite_f32(sum)) sum = plain_element<A_KC, B_KC>(g, row, col, 0, g.k);
+        finish_element(g, row, col, sum);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- small products
+// Outputs that fill few tiles: a workgroup owns a 32 x 32 tile and its wavefronts cut the contraction, each splitting its
+// fragments straight from memory in registers; their sums meet in LDS.  No barrier and no LDS in the loop, so a wavefront
+// keeps several steps' loads in flight, which is what such a product waits for.
+template <bool KC>
+__device__ __forceinline__ void direct_fragment(const float* __restrict__ p, int64_t ld, int64_t row, int64_t k, int64_t ke, bool vec,
+                                                float (&x)[8]) {
+    if (k + 8 <= ke) {
+        if (KC) {
+            const float* q = p + row * ld + k;
+            if (vec) {
+                const f32x4 u = *reinterpret_cast<const f32x4*>(q), v = *reinterpret_cast<const f32x4*>(q + 4);
+#pragma unroll
+                for (int e = 0; e < 4; e++) { x[e] = u[e]; x[4 + e] = v[e]; }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = q[e];
+            }
+        } else {
+            const float* q = p + k * ld + row;
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = q[e * ld];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = k + e < ke ? (KC ? p[row * ld + k + e] : p[(k + e) * ld + row]) : 0.f;
+    }
+}
+
+constexpr int kSmallWaves = 8;
+template <bool A_KC, bool B_KC>
+__global__ __launch_bounds__(64 * kSmallWaves) void epilogue_small_kernel(EpiArgs g, bool vec_a, bool vec_b) {
+    __shared__ float sums[kSmallWaves][32 * 33];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t m0 = (int64_t)(blockIdx.x / g.tiles_n) * 32, n0 = (int64_t)(blockIdx.x % g.tiles_n) * 32;
+    const int64_t kb = blockIdx.y * g.k_per_split, ke = min(g.k, kb + g.k_per_split);
+    const int64_t row = min(m0 + (lane & 31), g.m - 1), col = min(n0 + (lane & 31), g.n - 1);
+    f32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[e] = 0.f;
+    // kDepth steps' loads are issued before the first one's products
+    constexpr int kDepth = 2, kStep = 16 * kSmallWaves;
+    const int64_t half = 8 * (lane >> 5);
+    for (int64_t k = kb + 16 * wave; k < ke; k += kDepth * kStep) {
+        float x[kDepth][8], y[kDepth][8];
+#pragma unroll
+        for (int d = 0; d < kDepth; d++) {
+            direct_fragment<A_KC>(g.a, g.lda, row, k + d * kStep + half, ke, vec_a, x[d]);
+            direct_fragment<B_KC>(g.b, g.ldb, col, k + d * kStep + half, ke, vec_b, y[d]);
+        }
+#pragma unroll
+        for (int d = 0; d < kDepth; d++) {
+            u32x4 fa[kPlanes], fb[kPlanes];
+            split_eight(x[d], fa);
+            split_eight(y[d], fb);
+            acc = mfma_split(fa, fb, acc);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; e++) sums[wave][acc_row(e, lane) * 33 + (lane & 31)] = acc[e];
+    __syncthreads();
+    for (int i = tid; i < 32 * 32; i += 64 * kSmallWaves) {
+        const int64_t r = m0 + (i >> 5), c = n0 + (i & 31);
+        if (r >= g.m || c >= g.n) continue;
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kSmallWaves; w++) s += sums[w][(i >> 5) * 33 + (i & 31)];
+        if (g.splits > 1) {
+            g.partial[((int64_t)blockIdx.y * g.m + r) * g.n + c] = s;
+        } else {
+            if (!finite_f32(s)) s = plain_element<A_KC, B_KC>(g, r, c, 0, g.k);
+            finish_element(g, r, c, s);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- choice and launch
+static int g_force_variant = -1, g_force_splits = 0;
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename Cfg, bool A_KC, bool B_KC>
+static int launch_tile(const EpiArgs& g, bool va, bool vb, bool vc) {
+    constexpr int bytes = TileLds<Cfg, A_KC, B_KC>::BYTES;
+    static bool raised = false;                 // more than 64 KB of LDS has to be asked for once
+    if (!raised) {
+        const int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(&epilogue_tile_kernel<Cfg, A_KC, B_KC>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "bh_gemm_epilogue: LDS size");
+        if (rc) return rc;
+        raised = true;
+    }
+    hipLaunchKernelGGL((epilogue_tile_kernel<Cfg, A_KC, B_KC>), dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(Cfg::NT),
+                       bytes, stream(), g, va, vb, vc);
+    return BH_LAUNCH_CHECK("bh_gemm_epilogue");
+}
+
+enum { kTile256 = 0, kTile128 = 1, kSmall = 2 };
+
+template <bool A_KC, bool B_KC>
+static int run_product(EpiArgs g, int variant, int splits) {
+    const bool va = A_KC && g.lda % 4 == 0 && aligned16(g.a), vb = B_KC && g.ldb % 4 == 0 && aligned16(g.b);
+    const bool vc = g.ldc % 4 == 0 && aligned16(g.c) && (!g.saved || (g.lds % 4 == 0 && aligned16(g.saved))) &&
+                    (!g.residual || (g.ldr % 4 == 0 && aligned16(g.residual)));
+    const int bm = variant == kTile256 ? Tile256::BM : variant == kTile128 ? Tile128::BM : 32;
+    const int bn = variant == kTile256 ? Tile256::BN : variant == kTile128 ? Tile128::BN : 32;
+    const int64_t tiles_m = ceil_div(g.m, bm), tiles_n = ceil_div(g.n, bn);
+    if (tiles_m * tiles_n > 0x7fffffff) return set_error(BH_EINVAL, "bh_gemm_epilogue: output too large");
+    g.tiles_m = (int)tiles_m;
+    g.tiles_n = (int)tiles_n;
+    g.k_per_split = ceil_div(ceil_div(g.k > 0 ? g.k : 1, splits), 16) * 16;
+    g.splits = (int)ceil_div(g.k > 0 ? g.k : 1, g.k_per_split);
+    Scratch part;
+    if (g.splits > 1) {
+        if (!part.get(sizeof(float) * (size_t)g.splits * (size_t)(g.m * g.n))) return BH_ENOMEM;
+        g.partial = (float*)part.p;
+    }
+    int rc;
+    if (variant == kTile256) rc = launch_tile<Tile256, A_KC, B_KC>(g, va, vb, vc);
+    else if (variant == kTile128) rc = launch_tile<Tile128, A_KC, B_KC>(g, va, vb, vc);
+    else {
+        hipLaunchKernelGGL((epilogue_small_kernel<A_KC, B_KC>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)g.splits), dim3(64 * kSmallWaves), 0,
+                           stream(), g, va, vb);
+        rc = BH_LAUNCH_CHECK("bh_gemm_epilogue");
+    }
+    if (rc || g.splits == 1) return rc;
+    const int64_t blocks = ceil_div(g.m * g.n, 256);
+    hipLaunchKernelGGL((epilogue_fold_kernel<A_KC, B_KC>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream(), g);
+    return BH_LAUNCH_CHECK("bh_gemm_epilogue: fold");
+}
+
+static int product(int trans_a, int trans_b, EpiArgs g) {
+    int variant = g.m * g.n >= 128 * 128 * 64 ? kTile128 : kSmall, splits = 1;
+    if (g_force_variant >= 0) variant = g_force_variant;
+    if (g_force_splits > 0) splits = g_force_splits;
+    if (!trans_a) return trans_b ? run_product<true, true>(g, variant, splits) : run_product<true, false>(g, variant, splits);
+    return trans_b ? run_product<false, true>(g, variant, splits) : run_product<false, false>(g, variant, splits);
+}
+
+}  // namespace bh
+
+using namespace bh;
+
+extern "C" {
+
+int bh_gemm_epilogue(int trans_a, int trans_b, int64_t m, int64_t n, int64_t k, const float* a, int64_t lda, const float* b, int64_t ldb,
+                     float* c, int64_t ldc, const float* bias, int act, float* saved, int64_t lds, const float* residual, int64_t ldr) {
+    BH_CHECK_ARG(m >= 0 && n >= 0 && k >= 0, "negative dimension");
+    BH_CHECK_ARG(act >= BH_ACT_NONE && act <= BH_ACT_GELU, "unknown activation");
+    if (m == 0 || n == 0) return BH_OK;
+    BH_CHECK_ARG(c && ((a && b) || k == 0), "null pointer");
+    BH_CHECK_ARG(lda >= (trans_a ? m : k) && ldb >= (trans_b ? k : n) && ldc >= n, "leading dimension too small");
+    BH_CHECK_ARG((!saved || lds >= n) && (!residual || ldr >= n), "leading dimension too small");
+    BH_REQUIRE_INIT();
+    BH_CALL_GUARD();
+    ProfScope prof(BH_PROF_GEMM, 2.0 * (double)m * (double)n * (double)k);
+    EpiArgs g = {};
+    g.a = a; g.b = b; g.m = m; g.n = n; g.k = k; g.lda = lda; g.ldb = ldb; g.c = c; g.ldc = ldc; g.bias = bias;
+    g.saved = saved; g.lds = lds; g.residual = residual; g.ldr = ldr; g.act = act;
+    return product(trans_a, trans_b, g);
+}
+
+int bh_dense_act_backward(int act, const float* x, const float* w, const float* saved, const float* dy, float* dx, float* gw, float* gb,
+                          int64_t m, int64_t k, int64_t n, int accumulate) {
+    BH_CHECK_ARG(m >= 0 && k >= 0 && n >= 0, "negative dimension");
+    BH_CHECK_ARG(act >= BH_ACT_NONE && act <= BH_ACT_GELU, "unknown activation");
+    BH_CHECK_ARG((dy && (!dx || w) && (!gw || x) && (act == BH_ACT_NONE || saved)) || m == 0 || n == 0, "null pointer");
+    BH_REQUIRE_INIT();
+    BH_CALL_GUARD();
+    // dz = dy * act'(z), and with it db = its column sums
+    const float* dz = dy;
+    Scratch own;
+    int rc = BH_OK;
+    if (act != BH_ACT_NONE && m > 0 && n > 0 && (dx || gw || gb)) {
+        if (!own.get(sizeof(float) * (size_t)(m * n))) return BH_ENOMEM;
+        rc = gb ? bh_activation_backward_colsum(act, saved, dy, (float*)own.p, gb, m, n, accumulate)
+                : bh_activation_backward(act, saved, dy, (float*)own.p, m * n, 0);
+        dz = (const float*)own.p;
+    } else if (gb && n > 0) {
+        rc = m > 0 ? bh_colsum(dy, gb, m, n, accumulate) : accumulate ? BH_OK : bh_fill(gb, 0.f, n);
+    }
+    // dx[m,k] = dz[m,n] . w[k,n]^T     (n == 0: zeros)
+    if (rc == BH_OK && dx) rc = bh_gemm_epilogue(0, 1, m, k, n, dz, n, w, n, dx, k, nullptr, BH_ACT_NONE, nullptr, 0, nullptr, 0);
+    // gw[k,n] (+)= x[m,k]^T . dz[m,n]  (m == 0: zeros)
+    if (rc == BH_OK && gw)
+        rc = bh_gemm_epilogue(1, 0, k, n, m, x, k, dz, n, gw, n, nullptr, BH_ACT_NONE, nullptr, 0, accumulate ? gw : nullptr, n);
+    return rc;
+}
+
+int bh_gemm_epilogue_force(int variant, int splits) {
+    BH_CHECK_ARG(variant >= -1 && variant <= 2 && splits >= 0 && splits <= 64, "variant -1 to 2, 0 to 64 splits");
+    g_force_variant = variant;
+    g_force_splits = splits;
+    return BH_OK;
+}
+
+}  // extern "C"

@@ -84,6 +84,24 @@ void prof_close(int slot) {
     if (slot >= 0 && slot < (int)g_prof.size()) (void)hipEventRecord(g_prof[slot].b, g_stream);
 }
 
+constexpr int kDevice = 0;   // bh_init selects it
+
+CallGuard::CallGuard(const char* fn) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    rc = check_hip(hipStreamIsCapturing(g_stream, &status), fn);
+    if (!rc && status != hipStreamCaptureStatusNone)
+        rc = set_error(BH_EINVAL, "%s: cannot be captured into a graph (its work memory belongs to the library's cache)", fn);
+    int current = kDevice;
+    if (!rc) rc = check_hip(hipGetDevice(&current), fn);
+    if (!rc && current != kDevice) {
+        rc = check_hip(hipSetDevice(kDevice), fn);
+        if (!rc) previous = current;
+    }
+}
+CallGuard::~CallGuard() {
+    if (previous >= 0) (void)hipSetDevice(previous);
+}
+
 static size_t round_capacity(size_t n) {
     if (n == 0) n = 1;
     if (n <= (1u << 20)) return (n + 511) & ~size_t(511);          // 512 B granules below 1 MiB
@@ -103,10 +121,10 @@ int bh_init(void) {
     hipError_t e = hipGetDeviceCount(&n);
     if (e != hipSuccess || n < 1)
         return set_error(BH_EDEVICE, "bh_init: no HIP device visible (%s)", hipGetErrorString(e));
-    int rc = check_hip(hipSetDevice(0), "hipSetDevice");
+    int rc = check_hip(hipSetDevice(kDevice), "hipSetDevice");
     if (rc) return rc;
     hipDeviceProp_t prop;
-    rc = check_hip(hipGetDeviceProperties(&prop, 0), "hipGetDeviceProperties");
+    rc = check_hip(hipGetDeviceProperties(&prop, kDevice), "hipGetDeviceProperties");
     if (rc) return rc;
     snprintf(g_name, sizeof(g_name), "%s (%s)", prop.name, prop.gcnArchName);
     g_cus = prop.multiProcessorCount;

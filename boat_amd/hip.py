@@ -55,6 +55,9 @@ _SIGS = {
     "bh_softmax_ce_grad": (I, [P, P, P, P, L, L]),
     "bh_log_softmax_weighted_backward": (I, [P, P, P, P, P, L, L]),
     "bh_log_softmax_weighted_backward_colsum": (I, [P, P, P, P, P, P, L, L, I]),
+    "bh_distill_forward": (I, [P, L, P, P, P, L, L, L, F, F, F, P, P, P]),
+    "bh_distill_backward": (I, [P, L, P, P, P, L, L, L, F, F, F, P, P, P, L]),
+    "bh_distill_loss_grad": (I, [P, L, P, P, P, L, L, L, F, F, F, P, P, P, L]),
     "bh_layernorm_forward": (I, [P, P, P, P, P, P, L, L, F]),
     "bh_layernorm_backward": (I, [P, P, P, P, P, P, P, P, L, L, I]),
     "bh_layernorm_backward_add": (I, [P, P, P, P, P, P, P, P, P, L, L, I]),
@@ -68,6 +71,9 @@ _SIGS = {
     "bh_gemm_ksegments": (I, [I, I, L, L, L, I, C.POINTER(P), L, C.POINTER(P), L, P, L, P, I]),
     "bh_gemm_no_tables": (I, [I]),
     "bh_gemm_force_config": (I, [I]), "bh_gemm_force_direct": (I, [I]), "bh_gemm_force_splits": (I, [I]),
+    "bh_gemm_epilogue": (I, [I, I, L, L, L, P, L, P, L, P, L, P, I, P, L, P, L]),
+    "bh_dense_act_backward": (I, [I, P, P, P, P, P, P, P, L, L, L, I]),
+    "bh_gemm_epilogue_force": (I, [I, I]),
     "bh_transpose_last2": (I, [P, P, L, L, L]),
     "bh_dense_backward": (I, [P, P, P, P, P, P, L, L, L, I]),
     "bh_dense_backward_into": (I, [P, P, P, P, P, P, L, L, L, I, I]),
@@ -96,7 +102,7 @@ for _name, (_res, _args) in _SIGS.items():
     _fn.argtypes = _args
     globals()[_name] = _fn
 
-ACT_RELU, ACT_SIGMOID, ACT_TANH, ACT_GELU = 0, 1, 2, 3
+ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH, ACT_GELU = -1, 0, 1, 2, 3
 PROF_GEMM, PROF_SDPA_FWD, PROF_SDPA_BWD, PROF_NORM, PROF_OPTIMIZER, PROF_COLSUM = range(6)
 
 

@@ -104,6 +104,7 @@ int bh_scalar_op(int op, const float* a, float s, float* out, int64_t n);       
 /* d(a/b)/db = (dy*-1) * (a/(b*b))  (src/autodiff.c:1172-1201) */
 int bh_div_backward_b(const float* a, const float* b, const float* dy, float* db, int64_t n);
 
+#define BH_ACT_NONE   -1   /* the fused entry points only */
 #define BH_ACT_RELU    0
 #define BH_ACT_SIGMOID 1
 #define BH_ACT_TANH    2
@@ -165,6 +166,27 @@ int bh_log_softmax_weighted_backward_colsum(const float* y, const float* w, cons
  * dlogits = (softmax(z) - onehot)/B.  labels are class indices. */
 int bh_softmax_ce_grad(const float* logits, const int32_t* labels, float* dlogits, float* loss_out,
                        int64_t rows, int64_t cols);
+
+/* ---- distillation from a teacher's top logits (beside bh_softmax_ce_grad; no counterpart in the reference) ----
+ * logits [rows, vocab] (leading dimension ld); teacher and index [rows, topk]: the teacher's kept logits and the vocabulary
+ * entries they belong to, in any order, repeats allowed; labels [rows] or NULL.  An index outside [0, vocab) leaves its entry
+ * out, a label outside [0, vocab) leaves the row's label out.  With p = softmax(teacher / T) over a row's kept entries (a
+ * row without any, or with logits of -inf only, has no teacher part), q = softmax(logits / T) and r = softmax(logits):
+ *   row_loss = alpha T^2 sum_j p_j (log p_j - log q[index_j]) + (1 - alpha) (-log r[label]),   loss_out[0] = scale * sum of row_loss
+ *   dlogits  = seed * scale * (alpha T (q - p) + (1 - alpha) (r - onehot(label)))
+ * Without labels the second term is absent.  0 <= topk <= 4096, T > 0, alpha in [0, 1].  row_loss [rows], stats [3 * rows]
+ * and loss_out [1] may be NULL.  bh_distill_backward takes the stats of a forward call on the same arguments and seed (one
+ * float in device memory, NULL = 1); bh_distill_loss_grad is both passes in one (seed 1), reading the logits once.
+ * dlogits may be logits itself (ldd == ld); no other overlap. */
+int bh_distill_forward(const float* logits, int64_t ld, const float* teacher, const int32_t* index, const int32_t* labels,
+                       int64_t rows, int64_t vocab, int64_t topk, float temperature, float alpha, float scale,
+                       float* row_loss, float* stats, float* loss_out);
+int bh_distill_backward(const float* logits, int64_t ld, const float* teacher, const int32_t* index, const int32_t* labels,
+                        int64_t rows, int64_t vocab, int64_t topk, float temperature, float alpha, float scale,
+                        const float* stats, const float* seed, float* dlogits, int64_t ldd);
+int bh_distill_loss_grad(const float* logits, int64_t ld, const float* teacher, const int32_t* index, const int32_t* labels,
+                         int64_t rows, int64_t vocab, int64_t topk, float temperature, float alpha, float scale,
+                         float* row_loss, float* loss_out, float* dlogits, int64_t ldd);
 
 /* ---- LayerNorm (forward: src/layers/norm.c:184-317; backward: stub there, :397-402) ---- */
 int bh_layernorm_forward(const float* x, const float* gamma, const float* beta, float* y,
@@ -246,6 +268,23 @@ int bh_dense_backward(const float* x, const float* w, const float* dy,
 int bh_dense_backward_into(const float* x, const float* w, const float* dy,
                            float* dx, float* gw, float* gb, int64_t m, int64_t k, int64_t n,
                            int accumulate, int accumulate_dx);
+
+/* ---- a product that finishes its layer (a dense layer with activation and residual: src/layers/dense.c:135-188 and the
+ * elementwise passes behind it, src/autodiff.c:808-909, src/ops/arithmetic.c:197-282) ----
+ * z = op(A) . op(B) + bias[N];  C = act(z) + residual, row-major, operands and leading dimensions as bh_gemm, act one of
+ * BH_ACT_* or BH_ACT_NONE.  bias, saved and residual may be NULL.  saved [M,N] (leading dimension lds) receives what
+ * bh_activation_backward wants: z, or act(z) for BH_ACT_SIGMOID and BH_ACT_TANH.  residual [M,N] (ldr) may be C itself
+ * (C += act(z)); otherwise no output may overlap an operand.  K == 0: z = bias.
+ * fp32 sums on the bf16 matrix cores (each operand as the exact sum of three bf16, six partial products: the error of an
+ * fp32 product and sum); infinities and NaN come out as fp32 arithmetic gives them. */
+int bh_gemm_epilogue(int trans_a, int trans_b, int64_t m, int64_t n, int64_t k, const float* a, int64_t lda, const float* b,
+                     int64_t ldb, float* c, int64_t ldc, const float* bias, int act, float* saved, int64_t lds,
+                     const float* residual, int64_t ldr);
+/* Backward of y[m,n] = act(x[m,k] . w[k,n] + b) + residual, all dense: dz = dy * act'(saved); dx = dz . w^T (assigned),
+ * gw = x^T . dz and gb = column sums of dz (assigned, or added with accumulate != 0).  Any of dx, gw, gb may be NULL.  The
+ * residual's gradient is dy itself.  saved: as bh_gemm_epilogue left it (not read for BH_ACT_NONE). */
+int bh_dense_act_backward(int act, const float* x, const float* w, const float* saved, const float* dy, float* dx, float* gw,
+                          float* gb, int64_t m, int64_t k, int64_t n, int accumulate);
 
 /* ---- scaled dot-product attention on [bh, s, d] blocks (src/layers/attention.c:882-1079,1388-1534) ----
  * forward keeps O and the row log-sum-exp instead of the reference's [bh,s,s] softmax matrix;
@@ -333,6 +372,9 @@ int bh_gemm_force_splits(int splits);
  * where the shape allows) */
 int bh_gemm_no_tables(int off);
 int bh_sdpa_force_general(int on);
+/* bh_gemm_epilogue_force: variant 0 = 256x256, 1 = 128x128 tiles, 2 = 32x32 (small problems), -1 = by shape (default);
+ * splits > 0: cut the contraction this many ways, 0 = by shape */
+int bh_gemm_epilogue_force(int variant, int splits);
 /* bh_sdpa_force_wide: 1 = the attention backward's 256-key workgroups (eight wavefronts) wherever that form exists
  * (head_dim 32 and 64), 0 = never, -1 = chosen by shape (the default) */
 int bh_sdpa_force_wide(int mode);

@@ -1,0 +1,423 @@
+"""The fused training operators on the GPU against plain float64 forms: sizes at which tiles, segments and tails end, padded
+leading dimensions, empty rows, infinities, work split over the contraction, calls in place, from two threads and twice."""
+import ctypes as C
+import threading
+
+import numpy as np
+import pytest
+
+import operator_cases as oc
+from oracle_lib import fp32_gemm_bound, rel_fro
+
+pytestmark = pytest.mark.gpu
+
+_KEEP = []
+
+
+@pytest.fixture(autouse=True)
+def _release_device_arrays():
+    yield
+    _KEEP.clear()
+
+
+def dev(hip, a):
+    """Uploaded and kept until the test ends."""
+    if a is None:
+        return None
+    d = hip.to_device(np.ascontiguousarray(a))
+    _KEEP.append(d)
+    return d
+
+
+def ptr(d, elements=0):
+    return None if d is None else C.c_void_p(d.ptr + 4 * elements)
+
+
+def padded(a, ld, fill=np.nan):
+    """a [rows, cols] inside rows of ld floats."""
+    p = np.full((a.shape[0], ld), fill, np.float32)
+    p[:, :a.shape[1]] = a
+    return p
+
+
+# ------------------------------------------------------------------ product with epilogue
+
+def run_product(hip, a, b, ta, tb, act, bias, residual, keep, pad=0, in_place=False):
+    m, k = a.shape
+    n = b.shape[1]
+    sa, sb = (a.T if ta else a), (b.T if tb else b)
+    lda, ldb, ldc = sa.shape[1] + pad, sb.shape[1] + pad, n + pad
+    da, db = dev(hip, padded(sa, lda)), dev(hip, padded(sb, ldb))
+    dr = None if residual is None else dev(hip, padded(residual, ldc, 7.0))
+    dc = dr if in_place else dev(hip, np.full((m, ldc), 7.0, np.float32))
+    ds = dev(hip, np.full((m, ldc), 7.0, np.float32)) if keep else None
+    hip.check(hip.bh_gemm_epilogue(ta, tb, m, n, k, ptr(da), lda, ptr(db), ldb, ptr(dc), ldc, ptr(dev(hip, bias)), oc.ACTS[act],
+                                   ptr(ds), ldc, ptr(dr), ldc), "bh_gemm_epilogue")
+    c = dc.numpy()
+    assert (c[:, n:] == 7.0).all()                   # what lies between the rows stays
+    s = ds.numpy()[:, :n] if keep else None
+    return c[:, :n], s
+
+
+def check_product(hip, rng, m, n, k, ta, tb, act, with_bias, with_residual, keep, pad=0, in_place=False):
+    a, b = rng.standard_normal((m, k)).astype(np.float32), rng.standard_normal((k, n)).astype(np.float32)
+    bias = rng.standard_normal(n).astype(np.float32) if with_bias else None
+    residual = rng.standard_normal((m, n)).astype(np.float32) if with_residual else None
+    y, saved = run_product(hip, a, b, ta, tb, act, bias, residual, keep, pad, in_place)
+    a64, b64 = a.astype(np.float64), b.astype(np.float64)
+    z = a64 @ b64 + (bias if with_bias else 0)
+    want = oc.act(act, z) + (residual if with_residual else 0)
+    ez = oc.product_bound(a64, b64, 2 * oc.U * np.abs(z))
+    # every activation's slope is at most 1.13; its own evaluation is a handful of roundings of values up to |z| + 1
+    ey = 1.13 * ez + 16 * oc.U * (np.abs(z) + 1) + 2 * oc.U * np.abs(want)
+    assert (np.abs(y - want) <= ey).all(), np.max(np.abs(y - want) / ey)
+    if keep:
+        held = z if act in ("none", "relu", "gelu") else oc.act(act, z)
+        assert (np.abs(saved - held) <= ey).all()
+    if k > 0 and act == "none" and not with_residual:
+        assert rel_fro(y, want) <= fp32_gemm_bound(k)    # what narrower operands would fail
+
+
+@pytest.mark.parametrize("variant", [0, 1, 2])
+@pytest.mark.parametrize("ta,tb", [(0, 0), (0, 1), (1, 0), (1, 1)])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (33, 31, 17), (129, 257, 100), (256, 128, 64), (300, 140, 523)])
+def test_product_every_tile(hip, rng, variant, ta, tb, m, n, k):
+    hip.check(hip.bh_gemm_epilogue_force(variant, 0))
+    try:
+        check_product(hip, rng, m, n, k, ta, tb, "none", False, False, False, pad=0)
+        check_product(hip, rng, m, n, k, ta, tb, "gelu", True, True, True, pad=3)
+    finally:
+        hip.check(hip.bh_gemm_epilogue_force(-1, 0))
+
+
+@pytest.mark.parametrize("act", list(oc.ACTS))
+@pytest.mark.parametrize("variant", [0, 1, 2])
+def test_product_activations(hip, rng, act, variant):
+    hip.check(hip.bh_gemm_epilogue_force(variant, 0))
+    try:
+        check_product(hip, rng, 70, 132, 48, 0, 0, act, True, False, True, pad=4)
+        check_product(hip, rng, 260, 256, 32, 0, 1, act, False, True, True)
+    finally:
+        hip.check(hip.bh_gemm_epilogue_force(-1, 0))
+
+
+@pytest.mark.parametrize("variant,splits", [(0, 2), (0, 7), (1, 3), (2, 2), (2, 64)])
+@pytest.mark.parametrize("ta,tb", [(0, 0), (0, 1), (1, 0), (1, 1)])
+def test_product_split_contraction(hip, rng, variant, splits, ta, tb):
+    hip.check(hip.bh_gemm_epilogue_force(variant, splits))
+    try:
+        check_product(hip, rng, 130, 67, 333, ta, tb, "none", True, False, False)
+        check_product(hip, rng, 40, 130, 1000, ta, tb, "tanh", True, True, True, pad=1, in_place=True)
+        check_product(hip, rng, 5, 3, 9, ta, tb, "relu", True, True, True)      # fewer steps than splits
+    finally:
+        hip.check(hip.bh_gemm_epilogue_force(-1, 0))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 1024), (1, 5, 4000), (7, 1000, 784), (64, 128, 784), (500, 500, 500), (777, 513, 784), (2048, 1024, 256),
+                                   (1000, 1, 300), (4100, 3, 50)])
+def test_product_by_shape(hip, rng, m, n, k):
+    check_product(hip, rng, m, n, k, 0, 0, "none", True, False, False)
+    check_product(hip, rng, m, n, k, 1, 0, "gelu", True, True, True)
+    check_product(hip, rng, m, n, k, 0, 1, "none", True, True, False, in_place=True)
+
+
+def test_product_without_contraction_and_without_rows(hip, rng):
+    check_product(hip, rng, 5, 6, 0, 0, 0, "sigmoid", True, True, True)
+    d = dev(hip, np.full(8, 3.0, np.float32))
+    hip.check(hip.bh_gemm_epilogue(0, 0, 0, 4, 4, None, 4, ptr(d), 4, ptr(d), 4, None, -1, None, 0, None, 0))
+    assert (d.numpy() == 3.0).all()
+
+
+@pytest.mark.parametrize("variant,splits", [(0, 0), (1, 0), (2, 0), (1, 3)])
+def test_product_infinities_and_nan(hip, rng, variant, splits):
+    """What is not finite comes out as fp32 arithmetic gives it; the other rows and columns are untouched by it."""
+    hip.check(hip.bh_gemm_epilogue_force(variant, splits))
+    try:
+        a, b = rng.standard_normal((40, 70)).astype(np.float32), rng.standard_normal((70, 36)).astype(np.float32)
+        a[3, 5] = np.inf
+        a[7, 0] = np.nan
+        b[69, 11] = -np.inf
+        a[9, 9], b[9, 20] = 3.3999e38, 1e-3        # finite, but past the largest bf16
+        b[:, 30] = 0
+        for ta, tb in ((0, 0), (1, 0), (0, 1), (1, 1)):
+            y, _ = run_product(hip, a, b, ta, tb, "none", None, None, False)
+            with np.errstate(all="ignore"):
+                # in fp32 a product past the largest float is an infinity before the others are added to it
+                prod = a.astype(np.float64)[:, :, None] * b.astype(np.float64)[None]
+                prod = np.where(np.abs(prod) > 3.4028235e38, np.sign(prod) * np.inf, prod)
+                want = prod.sum(1)
+            assert (np.isnan(y) == np.isnan(want)).all(), np.argwhere(np.isnan(y) != np.isnan(want))
+            assert (y[np.isinf(want)] == want[np.isinf(want)]).all()
+            ok = np.isfinite(want)
+            assert (np.abs(y - want)[ok] <= 200 * oc.U * (np.abs(np.nan_to_num(a, posinf=0, neginf=0)).astype(np.float64)
+                                                          @ np.abs(np.nan_to_num(b, posinf=0, neginf=0)) + 1e-30)[ok]).all()
+    finally:
+        hip.check(hip.bh_gemm_epilogue_force(-1, 0))
+
+
+@pytest.mark.parametrize("scale_a,scale_b", [(1e-30, 1e30), (1e-36, 1e20), (1e18, 1e18), (1e-20, 1e-19)])
+def test_product_over_the_exponent_range(hip, rng, scale_a, scale_b):
+    a = (rng.standard_normal((33, 40)) * scale_a).astype(np.float32)
+    b = (rng.standard_normal((40, 35)) * scale_b).astype(np.float32)
+    y, _ = run_product(hip, a, b, 0, 0, "none", None, None, False)
+    a64, b64 = a.astype(np.float64), b.astype(np.float64)
+    # below 2^-110 a value's last part is a subnormal bf16, off by half of 2^-133 at most, against the other operand
+    tail = 2.0 ** -133 * (np.abs(b64).sum(0)[None] + np.abs(a64).sum(1)[:, None]) + 2.0 ** -126
+    assert (np.abs(y - a64 @ b64) <= oc.product_bound(a64, b64) + tail).all()
+
+
+def test_product_twice_is_the_same_and_threads_do_not_mix(hip, rng):
+    a, b = rng.standard_normal((300, 1000)).astype(np.float32), rng.standard_normal((1000, 200)).astype(np.float32)
+    first = run_product(hip, a, b, 0, 0, "gelu", None, None, True)
+    again = run_product(hip, a, b, 0, 0, "gelu", None, None, True)
+    assert np.array_equal(first[0], again[0]) and np.array_equal(first[1], again[1])
+    da, db = dev(hip, a), dev(hip, b)
+    outs = [dev(hip, np.zeros((300, 200), np.float32)) for _ in range(8)]
+    rcs = []
+
+    def call(o):
+        for _ in range(10):
+            rcs.append(hip.bh_gemm_epilogue(0, 0, 300, 200, 1000, ptr(da), 1000, ptr(db), 200, ptr(o), 200, None, 3, None, 0, None, 0))
+    threads = [threading.Thread(target=call, args=(o,)) for o in outs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert rcs == [0] * 80
+    for o in outs:
+        assert np.array_equal(o.numpy(), first[0])
+
+
+@pytest.mark.parametrize("act", list(oc.ACTS))
+@pytest.mark.parametrize("m,k,n", [(1, 5, 3), (64, 784, 128), (333, 130, 65), (1000, 256, 300)])
+def test_dense_backward(hip, rng, act, m, k, n):
+    x, w = rng.standard_normal((m, k)).astype(np.float32), (rng.standard_normal((k, n)) / np.sqrt(k)).astype(np.float32)
+    b, dy = rng.standard_normal(n).astype(np.float32), rng.standard_normal((m, n)).astype(np.float32)
+    dx_, dw_, db_, ddy = dev(hip, x), dev(hip, w), dev(hip, b), dev(hip, dy)
+    y, saved = hip.empty((m, n)), hip.empty((m, n))
+    hip.check(hip.bh_gemm_epilogue(0, 0, m, n, k, ptr(dx_), k, ptr(dw_), n, ptr(y), n, ptr(db_), oc.ACTS[act], ptr(saved), n, None, 0))
+    gx = dev(hip, np.full((m, k), np.nan, np.float32))
+    gw, gb = dev(hip, np.full((k, n), np.nan, np.float32)), dev(hip, np.full(n, np.nan, np.float32))
+    call = (oc.ACTS[act], ptr(dx_), ptr(dw_), ptr(saved), ptr(ddy), ptr(gx), ptr(gw), ptr(gb), m, k, n)
+    hip.check(hip.bh_dense_act_backward(*call, 0))
+    x64, w64 = x.astype(np.float64), w.astype(np.float64)
+    z = x64 @ w64 + b
+    dz = dy * oc.act_slope(act, z)
+    # dz: the saved value's error (z's bound) times a second derivative of at most 1.2, and ten roundings; a ReLU's sign may
+    # turn where z is as small as its bound
+    ez = oc.product_bound(x64, w64, 2 * oc.U * np.abs(z))
+    edz = np.abs(dy) * (1.2 * ez + 16 * oc.U) + (np.abs(dy) * (np.abs(z) <= ez) if act == "relu" else 0)
+    ex = oc.product_bound(dz, w64.T) + edz @ np.abs(w64).T
+    ew = oc.product_bound(x64.T, dz) + np.abs(x64).T @ edz
+    eb = 2 * m * oc.U * np.abs(dz).sum(0) + edz.sum(0)
+    first = [gx.numpy(), gw.numpy(), gb.numpy()]
+    for got, want, bound in zip(first, (dz @ w64.T, x64.T @ dz, dz.sum(0)), (ex, ew, eb)):
+        assert (np.abs(got - want) <= bound + 1e-30).all()
+    hip.check(hip.bh_dense_act_backward(*call, 1))           # dx assigned, gw and gb added to
+    assert np.array_equal(gx.numpy(), first[0])
+    assert (np.abs(gw.numpy() - 2 * first[1].astype(np.float64)) <= 4 * oc.U * np.abs(first[1])).all()
+    assert (np.abs(gb.numpy() - 2 * first[2].astype(np.float64)) <= 2 * eb + 4 * oc.U * np.abs(first[2])).all()
+    for drop in (5, 6, 7):                                   # any of the three may be left out
+        part = list(call)
+        part[drop] = None
+        hip.check(hip.bh_dense_act_backward(*part, 0))
+    assert np.array_equal(gx.numpy(), first[0])
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "tanh", "gelu"])
+def test_dense_backward_against_differences(hip, rng, act):
+    m, k, n = 9, 20, 7
+    x, w, b = rng.standard_normal((m, k)), rng.standard_normal((k, n)) / 4, rng.standard_normal(n)
+    x, w, b = (t.astype(np.float32) for t in (x, w, b))
+    dy = rng.standard_normal((m, n)).astype(np.float32)
+    args = [dev(hip, t) for t in (x, w, b, dy)]
+    y, saved, gx, gw, gb = hip.empty((m, n)), hip.empty((m, n)), hip.empty((m, k)), hip.empty((k, n)), hip.empty(n)
+    hip.check(hip.bh_gemm_epilogue(0, 0, m, n, k, ptr(args[0]), k, ptr(args[1]), n, ptr(y), n, ptr(args[2]), oc.ACTS[act], ptr(saved), n, None, 0))
+    hip.check(hip.bh_dense_act_backward(oc.ACTS[act], ptr(args[0]), ptr(args[1]), ptr(saved), ptr(args[3]), ptr(gx), ptr(gw), ptr(gb), m, k, n, 0))
+
+    def loss(x, w, b):
+        return float((oc.act(act, x.astype(np.float64) @ w + b) * dy).sum())
+    eps = 1e-5
+    for grad, at in ((gx.numpy(), 0), (gw.numpy(), 1), (gb.numpy(), 2)):
+        d = rng.standard_normal(grad.shape)
+        up, down = [x, w, b], [x, w, b]
+        up[at], down[at] = up[at] + eps * d, down[at] - eps * d
+        diff = (loss(*up) - loss(*down)) / (2 * eps)
+        # differences: eps^2 of third derivatives (1e-10 times a few hundred) and 1e-16 / eps of rounding, times sum |terms|
+        assert abs(float((grad * d).sum()) - diff) <= 1e-5 * float(np.abs(grad * d).sum() + 1)
+
+
+def test_dense_backward_of_nothing(hip):
+    gw, gb = dev(hip, np.full((3, 2), 5.0, np.float32)), dev(hip, np.full(2, 5.0, np.float32))
+    hip.check(hip.bh_dense_act_backward(3, None, None, None, None, None, ptr(gw), ptr(gb), 0, 3, 2, 1))
+    assert (gw.numpy() == 5.0).all() and (gb.numpy() == 5.0).all()
+    hip.check(hip.bh_dense_act_backward(3, None, None, None, None, None, ptr(gw), ptr(gb), 0, 3, 2, 0))
+    assert (gw.numpy() == 0).all() and (gb.numpy() == 0).all()
+
+
+# ------------------------------------------------------------------ distillation
+
+def distill_case(rng, rows, vocab, topk, labels=True):
+    z = (2.5 * rng.standard_normal((rows, vocab))).astype(np.float32)
+    teacher = (3 * rng.standard_normal((rows, topk))).astype(np.float32)
+    index = rng.integers(0, vocab, (rows, topk)).astype(np.int32)            # repeats among them
+    if topk:
+        index[rng.random((rows, topk)) < 0.15] = -1
+        index[rows // 2] = -1                                                # a row with nothing kept
+        index[rows // 3, 0] = vocab + 3                                      # past the vocabulary: left out
+        index[-1] = index[-1, 0]                                             # one entry many times over
+        teacher[0, 0] = -np.inf
+    lab = rng.integers(0, vocab, rows).astype(np.int32) if labels else None
+    if labels:
+        lab[0] = -1
+        if topk and index[-1, 0] >= 0:
+            lab[-1] = min(index[-1, 0], vocab - 1)                           # the label among the teacher's entries
+    return z, teacher, index, lab
+
+
+def run_distill(hip, z, teacher, index, labels, temperature, alpha, scale, pad=0, shift=0, in_place=False):
+    rows, vocab = z.shape
+    ld = vocab + pad
+    flat = np.full(rows * ld + shift + 4, 9.0, np.float32)
+    flat[shift:shift + rows * ld].reshape(rows, ld)[:, :vocab] = z
+    dz_flat = np.full_like(flat, 9.0)
+    dl = dev(hip, flat)
+    dg = dl if in_place else dev(hip, dz_flat)
+    row, stats, loss = hip.zeros(max(rows, 1)), hip.zeros(3 * max(rows, 1)), hip.zeros(1)
+    head = (ptr(dl, shift), ld, ptr(dev(hip, teacher)), ptr(dev(hip, index)), ptr(dev(hip, labels)), rows, vocab, teacher.shape[1],
+            temperature, alpha, scale)
+    hip.check(hip.bh_distill_forward(*head, ptr(row), ptr(stats), ptr(loss)), "bh_distill_forward")
+    forward = row.numpy()[:rows], float(loss.numpy()[0])
+    seed = dev(hip, np.array([2.0], np.float32))
+    if not in_place:
+        hip.check(hip.bh_distill_backward(*head, ptr(stats), ptr(seed), ptr(dg, shift), ld), "bh_distill_backward")
+        flat_back = dg.numpy()
+    hip.check(hip.bh_distill_loss_grad(*head, ptr(row), ptr(loss), ptr(dg, shift), ld), "bh_distill_loss_grad")
+    both = row.numpy()[:rows], float(loss.numpy()[0])
+    out = dg.numpy()
+    inner = out[shift:shift + rows * ld].reshape(rows, ld)
+    assert (inner[:, vocab:] == 9.0).all() and (out[:shift] == 9.0).all() and (out[shift + rows * ld:] == 9.0).all()
+    back = None if in_place else flat_back[shift:shift + rows * ld].reshape(rows, ld)[:, :vocab]
+    return forward, both, inner[:, :vocab], back
+
+
+def check_distill(hip, z, teacher, index, labels, temperature, alpha, pad=0, shift=0, in_place=False):
+    scale = 1.0 / z.shape[0]
+    want_row, want_loss, want_dz = oc.distill(z, teacher, index, labels, temperature, alpha, scale)
+    tol_row, tol_dz = oc.distill_bounds(z, teacher, temperature, alpha, scale)
+    (row, loss), (row2, loss2), dz, back = run_distill(hip, z, teacher, index, labels, temperature, alpha, scale, pad, shift, in_place)
+    for r in (row, row2):
+        assert (np.abs(r - want_row) <= tol_row + 4 * oc.U * np.abs(want_row)).all(), np.abs(r - want_row).max() / tol_row
+    for l in (loss, loss2):
+        assert abs(l - want_loss) <= tol_row + 4 * oc.U * abs(want_loss)
+    assert (np.abs(dz - want_dz) <= tol_dz).all(), np.abs(dz - want_dz).max() / tol_dz
+    if back is not None:
+        assert (np.abs(back - 2 * want_dz) <= 2 * tol_dz).all()
+        # a dense part that is relatively as good: far from the special places the gradient is a softmax value
+        big = np.abs(want_dz) > 1e-12
+        assert rel_fro(dz[big], want_dz[big]) <= 4e-6
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 3, 5, 64, 1000, 1024, 1025, 4096, 4099])
+@pytest.mark.parametrize("rows,topk", [(1, 1), (5, 8), (300, 3)])
+def test_distill_small_vocabularies(hip, rng, rows, topk, vocab):
+    check_distill(hip, *distill_case(rng, rows, vocab, topk), 2.0, 0.6)
+
+
+@pytest.mark.parametrize("rows,vocab,topk", [(257, 16385, 5), (256, 32771, 7), (256, 70003, 4), (3, 70003, 64), (1, 131072, 200), (37, 9001, 16),
+                                             (2, 8192, 1)])
+def test_distill_large_vocabularies(hip, rng, rows, vocab, topk):
+    check_distill(hip, *distill_case(rng, rows, vocab, topk), 3.0, 0.8, pad=3 if rows < 100 else 0)
+
+
+@pytest.mark.parametrize("temperature", [0.25, 1.0, 8.0])
+@pytest.mark.parametrize("alpha", [0.0, 0.5, 1.0])
+@pytest.mark.parametrize("labels", [True, False])
+def test_distill_mixtures(hip, rng, temperature, alpha, labels):
+    check_distill(hip, *distill_case(rng, 7, 777, 9, labels), temperature, alpha, pad=5, shift=1)
+
+
+@pytest.mark.parametrize("rows,vocab", [(4, 1001), (3, 20001), (300, 2050), (256, 66000)])
+def test_distill_gradient_in_place(hip, rng, rows, vocab):
+    check_distill(hip, *distill_case(rng, rows, vocab, 12), 2.0, 0.5, in_place=True)
+
+
+def test_distill_backward_in_place_over_segments(hip, rng):
+    rows, vocab, topk = 3, 40001, 30
+    z, teacher, index, labels = distill_case(rng, rows, vocab, topk)
+    apart = run_distill(hip, z, teacher, index, labels, 2.0, 0.5, 1.0)
+    dl, stats, loss = dev(hip, z), hip.zeros(3 * rows), hip.zeros(1)
+    head = (ptr(dl), vocab, ptr(dev(hip, teacher)), ptr(dev(hip, index)), ptr(dev(hip, labels)), rows, vocab, topk, 2.0, 0.5, 1.0)
+    hip.check(hip.bh_distill_forward(*head, None, ptr(stats), ptr(loss)))
+    seed = dev(hip, np.array([2.0], np.float32))
+    hip.check(hip.bh_distill_backward(*head, ptr(stats), ptr(seed), ptr(dl), vocab))
+    assert np.array_equal(dl.numpy(), apart[3])
+
+
+def test_distill_without_teacher_is_cross_entropy(hip, rng):
+    z, _, _, labels = distill_case(rng, 20, 333, 1)
+    check_distill(hip, z, np.zeros((20, 0), np.float32), np.zeros((20, 0), np.int32), labels, 1.0, 0.0)
+
+
+@pytest.mark.parametrize("rows,vocab", [(4, 100), (2, 20000)])
+def test_distill_masked_logits(hip, rng, rows, vocab):
+    """A vocabulary entry masked with -inf or with the lowest float has no probability and no gradient."""
+    z, teacher, index, labels = distill_case(rng, rows, vocab, 6)
+    z[:, ::3] = -np.inf
+    z[:, 1::3] = np.finfo(np.float32).min
+    z[:, 2] = 1.0
+    index = np.where(index >= 0, index - index % 3 + 2, index)
+    index[index >= vocab] = 2
+    labels = np.where(labels >= 0, 2, labels).astype(np.int32)
+    scale = 1.0 / rows
+    want_row, _, want_dz = oc.distill(z, teacher, index, labels, 2.0, 0.5, scale)
+    (row, _), _, dz, _ = run_distill(hip, z, teacher, index.astype(np.int32), labels, 2.0, 0.5, scale)
+    tol_row, tol_dz = oc.distill_bounds(np.where(z < -1e30, 0, z), teacher, 2.0, 0.5, scale)
+    assert (np.abs(row - want_row) <= tol_row).all() and (np.abs(dz - want_dz) <= tol_dz).all()
+    assert (dz[:, ::3] == 0).all() and (dz[:, 1::3] == 0).all()
+
+
+def test_distill_no_rows(hip):
+    loss = dev(hip, np.array([5.0], np.float32))
+    hip.check(hip.bh_distill_forward(None, 10, None, None, None, 0, 10, 3, 1.0, 1.0, 1.0, None, None, ptr(loss)))
+    assert loss.numpy()[0] == 0
+    hip.check(hip.bh_distill_backward(None, 10, None, None, None, 0, 10, 3, 1.0, 1.0, 1.0, None, None, None, 10))
+
+
+def test_distill_against_differences(hip, rng):
+    rows, vocab, topk = 6, 40, 5
+    z, teacher, index, labels = distill_case(rng, rows, vocab, topk)
+    _, _, dz, _ = run_distill(hip, z, teacher, index, labels, 1.5, 0.4, 1.0)
+    d = rng.standard_normal(z.shape)
+    eps = 1e-5
+    up = oc.distill(z + eps * d, teacher, index, labels, 1.5, 0.4, 1.0)[1]
+    down = oc.distill(z - eps * d, teacher, index, labels, 1.5, 0.4, 1.0)[1]
+    # eps^2 times third derivatives of order one, 1e-16 |loss| / eps of rounding, and the gradient's own bound
+    assert abs(float((dz * d).sum()) - (up - down) / (2 * eps)) <= 1e-6 + oc.distill_bounds(z, teacher, 1.5, 0.4, 1.0)[1] * np.abs(d).sum()
+
+
+def test_distill_twice_is_the_same(hip, rng):
+    case = distill_case(rng, 5, 30000, 40)
+    one, two = (run_distill(hip, *case, 2.0, 0.5, 0.2) for _ in range(2))
+    assert np.array_equal(one[0][0], two[0][0]) and one[0][1] == two[0][1] and np.array_equal(one[2], two[2]) and np.array_equal(one[3], two[3])
+
+
+# ------------------------------------------------------------------ all of them
+
+def test_capture_is_refused(hip):
+    """Work memory comes from the library's cache, so a call on a capturing stream is refused before it queues anything."""
+    rt = hip.lib        # the runtime the library is linked to: its symbols are found through the library
+    graph = C.c_void_p()
+    d = dev(hip, np.ones(64, np.float32))
+    i = dev(hip, np.zeros(64, np.int32))
+    assert rt.hipStreamBeginCapture(C.c_void_p(hip.bh_stream()), 2) == 0
+    try:
+        rcs = [hip.bh_gemm_epilogue(0, 0, 4, 4, 4, ptr(d), 4, ptr(d), 4, ptr(d, 32), 4, None, -1, None, 0, None, 0),
+               hip.bh_distill_forward(ptr(d), 8, ptr(d), ptr(i), None, 2, 8, 2, 1.0, 1.0, 1.0, None, None, ptr(d, 32))]
+        text = hip.bh_last_error().decode()
+    finally:
+        assert rt.hipStreamEndCapture(C.c_void_p(hip.bh_stream()), C.byref(graph)) == 0
+        if graph:
+            rt.hipGraphDestroy(graph)
+    assert rcs == [-1, -1] and "captured" in text
+    assert (d.numpy() == 1).all()
