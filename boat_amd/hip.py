@@ -21,6 +21,15 @@ if not LIB_PATH.exists():
     raise FileNotFoundError(f"{LIB_PATH} not found: build it first (python -m boat_amd.build); there is no host fallback")
 lib = C.CDLL(str(LIB_PATH), mode=C.RTLD_LOCAL)
 
+
+
+class RelbiasAttention(C.Structure):
+    """bh_relbias_attention_t."""
+    _fields_ = [(n, L) for n in ("batch", "heads", "kv_heads", "sq", "sk", "d")] + [
+        (n, L * 3) for n in ("q_stride", "k_stride", "v_stride", "o_stride")] + [("query_offset", L)] + [
+        (n, C.c_int32) for n in ("num_buckets", "max_distance", "bidirectional", "causal")] + [("scale", F)]
+
+
 _SIGS = {
     "bh_init": (I, []), "bh_shutdown": (I, []), "bh_synchronize": (I, []),
     "bh_last_error": (C.c_char_p, []), "bh_device_name": (C.c_char_p, []), "bh_device_cu_count": (I, []),
@@ -83,6 +92,10 @@ _SIGS = {
     "bh_sdpa_score_cache_bytes": (C.c_size_t, [L, L, L]),
     "bh_sdpa_forward_cached": (I, [P, P, P, F, I, P, P, P, L, L, L]),
     "bh_sdpa_backward_cached": (I, [P, P, P, P, P, P, P, F, I, P, P, P, L, L, L]),
+    "bh_relative_position_bucket": (I, [L, I, I, I]),
+    "bh_relbias_attention_force_rows": (I, [I]),
+    "bh_relbias_attention_forward": (I, [C.POINTER(RelbiasAttention)] + [P] * 7),
+    "bh_relbias_attention_backward": (I, [C.POINTER(RelbiasAttention)] + [P] * 12 + [I]),
     "bh_adam_update": (I, [P, P, P, P, L, F, F, F, F, L]),
     "bh_stream_probe_4r3w": (I, [P, P, P, P, L]),
     "bh_conv2d_forward": (I, [P, P, P, P] + [L] * 8),
@@ -104,6 +117,12 @@ for _name, (_res, _args) in _SIGS.items():
 
 ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH, ACT_GELU = -1, 0, 1, 2, 3
 PROF_GEMM, PROF_SDPA_FWD, PROF_SDPA_BWD, PROF_NORM, PROF_OPTIMIZER, PROF_COLSUM = range(6)
+
+
+def relbias_attention(*, q_stride, k_stride, v_stride, o_stride, **rest) -> RelbiasAttention:
+    """The description both directions of bh_relbias_attention take; strides are (batch, head, row) in elements."""
+    return RelbiasAttention(q_stride=(L * 3)(*q_stride), k_stride=(L * 3)(*k_stride), v_stride=(L * 3)(*v_stride),
+                            o_stride=(L * 3)(*o_stride), **rest)
 
 
 def profile_read(cls):

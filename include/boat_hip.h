@@ -307,6 +307,36 @@ int bh_sdpa_backward_cached(const float* q, const float* k, const float* v, cons
                             const float* scores, const float* d_out, float scale, int causal,
                             float* dq, float* dk, float* dv, int64_t bh, int64_t s, int64_t d);
 
+/* ---- attention with a learned relative position bias by buckets (the attention core above, src/layers/attention.c:882-1079,
+ * with a bias the reference does not have) ----
+ *   x = scale q_i . k_j + table[bucket(j - (i + query_offset))][head],  out = softmax_j(x) v,  lse = log sum_j exp(x)
+ * Buckets of a relative position r = key - query: of the num_buckets (per direction half of them when bidirectional: the
+ * second half for r > 0; otherwise r > 0 counts as 0), the first half of a direction's are the distances 0, 1, 2, ... and
+ * the rest grow logarithmically up to max_distance: with e = half, n >= e falls into e + floor(log(n/e) / log(max_distance/e)
+ * * (count - e)), at most the last.  table [num_buckets, heads], dense; a value of -1e30 or less masks its bucket.
+ * Operands are [batch, heads, rows, d] by strides of batch, head and row in elements (d contiguous; any order of the three);
+ * heads is a multiple of kv_heads, head h reads key head h / (heads / kv_heads); 1 <= d <= 128; 2 to 256 buckets.
+ * kv_len [batch] (or NULL) holds the number of valid keys of each sequence, values outside [0, sk] counting as the nearer
+ * end: what lies behind them is not read.  causal: a query sees keys with r <= 0 only.  A query that sees no key has out = 0,
+ * lse = -inf and no gradient.  lse [batch, heads, sq], dense. */
+typedef struct bh_relbias_attention {
+    int64_t batch, heads, kv_heads, sq, sk, d;
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+    int64_t query_offset;      /* position of query 0 counted from key 0: sk - sq where the queries are the last tokens */
+    int32_t num_buckets, max_distance, bidirectional, causal;
+    float scale;
+} bh_relbias_attention_t;
+/* the bucket of one relative position (host arithmetic), or BH_EINVAL */
+int bh_relative_position_bucket(int64_t relative, int num_buckets, int max_distance, int bidirectional);
+int bh_relbias_attention_forward(const bh_relbias_attention_t* p, const float* q, const float* k, const float* v,
+                                 const float* table, const int32_t* kv_len, float* out, float* lse);
+/* out and lse: of the forward call.  d_out has the strides of out; dq, dk, dv those of q, k, v (assigned; zero at keys behind
+ * kv_len; the heads that share a key head add up); dtable [num_buckets, heads] is assigned, or added to with
+ * accumulate_table != 0.  The same inputs give the same bits every time. */
+int bh_relbias_attention_backward(const bh_relbias_attention_t* p, const float* q, const float* k, const float* v,
+                                  const float* table, const int32_t* kv_len, const float* out, const float* lse,
+                                  const float* d_out, float* dq, float* dk, float* dv, float* dtable, int accumulate_table);
+
 /* ---- 2-D convolution and max pooling, NCHW, square kernel/window (src/layers/conv.c:46-201,326-437; src/layers/pool.c:63-218) ----
  * x [batch, in_channels, height, width]; w [out_channels, in_channels, kernel, kernel]; bias [out_channels] or NULL;
  * y / dy [batch, out_channels, ho, wo] with ho = (height + 2*pad - kernel)/stride + 1.
@@ -372,6 +402,8 @@ int bh_gemm_force_splits(int splits);
  * where the shape allows) */
 int bh_gemm_no_tables(int off);
 int bh_sdpa_force_general(int on);
+/* bh_relbias_attention_force_rows: 1 = the forward pass's kernel for few query rows, 0 = its tiles, -1 = by shape (default) */
+int bh_relbias_attention_force_rows(int mode);
 /* bh_gemm_epilogue_force: variant 0 = 256x256, 1 = 128x128 tiles, 2 = 32x32 (small problems), -1 = by shape (default);
  * splits > 0: cut the contraction this many ways, 0 = by shape */
 int bh_gemm_epilogue_force(int variant, int splits);

@@ -84,3 +84,80 @@ def distill_bounds(z, teacher, temperature, alpha, scale):
     logs = spread + spread_t + math.log(vocab + 1) + 10
     row = (alpha * temperature ** 2 + 1 - alpha) * (rel + 8 * U * logs) * 2
     return row, scale * (alpha * temperature + 1 - alpha) * rel * 2
+
+
+# ------------------------------------------------------------------ attention with a relative position bias
+
+def bucket(rel, buckets, distance, both):
+    """The bucket of one relative position, the logarithm's borders decided in whole numbers."""
+    first = 0
+    if both:
+        buckets //= 2
+        first, n = (buckets if rel > 0 else 0), abs(rel)
+    else:
+        n = max(-rel, 0)
+    e = buckets // 2
+    if n < e:
+        return first + n
+    if n >= distance:
+        return first + buckets - 1
+    j = 0
+    while j + 1 < buckets - e and n ** (buckets - e) * e ** (j + 1) >= distance ** (j + 1) * e ** (buckets - e):
+        j += 1
+    return first + e + j
+
+
+def attention(q, k, v, table, lens, offset, buckets, distance, both, causal, scale, d_out=None):
+    """[batch, heads, rows, d] arrays; returns out, lse and, with d_out, dq, dk, dv, dtable, each with a bound on its rounding error."""
+    batch, heads, sq, d = q.shape
+    kv_heads, sk = k.shape[1:3]
+    group = heads // kv_heads
+    rel = np.arange(sk)[None] - (np.arange(sq)[:, None] + offset)
+    lut = {r: bucket(int(r), buckets, distance, both) for r in np.unique(rel)}
+    idx = np.array([[lut[r] for r in row] for row in rel], dtype=np.int64).reshape(sq, sk)
+    z = {n: np.zeros(a.shape) for n, a in (("out", q), ("dq", q), ("dk", k), ("dv", v), ("dtable", table))}
+    e = {n: np.zeros(a.shape) for n, a in z.items()}
+    z["lse"], e["lse"] = np.full((batch, heads, sq), -np.inf), np.zeros((batch, heads, sq))
+    for b in range(batch):
+        seen = np.broadcast_to(np.arange(sk)[None] < (sk if lens is None else min(max(int(lens[b]), 0), sk)), (sq, sk))
+        if causal:
+            seen = seen & (rel <= 0)
+        some = seen.any(1)
+        for h in range(heads):
+            K = np.where(seen.any(0)[:, None], k[b, h // group], 0).astype(np.float64) if lens is not None else k[b, h // group].astype(np.float64)
+            V = np.where(seen.any(0)[:, None], v[b, h // group], 0).astype(np.float64) if lens is not None else v[b, h // group].astype(np.float64)
+            Q = q[b, h].astype(np.float64)
+            bias = np.where(table[:, h] <= -1e30, -np.inf, table[:, h].astype(np.float64))[idx]
+            x = np.where(seen, scale * (Q @ K.T) + bias, -np.inf)
+            alive = some & (x.max(1, initial=-np.inf) > -np.inf)
+            m = np.where(alive, x.max(1, initial=-np.inf), 0)
+            p = np.exp(x - m[:, None])
+            total = p.sum(1)
+            p = p / np.where(alive, total, 1)[:, None]
+            z["out"][b, h] = p @ V
+            z["lse"][b, h] = np.where(alive, m + np.log(np.where(alive, total, 1)), -np.inf)
+            # scores: the product's bound and four roundings; a probability twice that (numerator and sum) and the exponential's
+            ex = abs(scale) * product_bound(Q, K.T) + 4 * U * (np.abs(np.where(seen & np.isfinite(x), x, 0)) + np.abs(m)[:, None])
+            ex = np.where(seen, ex, 0).max(1, initial=0)[:, None]
+            rel_p = 2 * ex + (2 * sk + 16) * U
+            e["out"][b, h] = (rel_p + (2 * sk + 8) * U) * (p @ np.abs(V))
+            e["lse"][b, h] = (ex + (2 * sk + 8) * U)[:, 0] + 4 * U * np.abs(np.where(alive, z["lse"][b, h], 0))
+            if d_out is None:
+                continue
+            G = d_out[b, h].astype(np.float64)
+            rel_p = rel_p + 8 * U * np.abs(np.where(alive, z["lse"][b, h], 0))[:, None]
+            dp = G @ V.T
+            delta = (p * dp).sum(1)[:, None]
+            ds = p * (dp - delta)
+            e_delta = (2 * d + 4) * U * (np.abs(G) * np.abs(z["out"][b, h])).sum(1)[:, None] + (np.abs(G) * e["out"][b, h]).sum(1)[:, None]
+            e_ds = p * (rel_p * np.abs(dp - delta) + product_bound(G, V.T) + e_delta + 4 * U * (np.abs(dp) + np.abs(delta)))
+            z["dq"][b, h] = scale * (ds @ K)
+            e["dq"][b, h] = abs(scale) * (e_ds @ np.abs(K) + product_bound(ds, K)) * (1 + 4 * U)
+            z["dk"][b, h // group] += scale * (ds.T @ Q)
+            e["dk"][b, h // group] += abs(scale) * (e_ds.T @ np.abs(Q) + group * product_bound(ds.T, Q))
+            z["dv"][b, h // group] += p.T @ G
+            e["dv"][b, h // group] += (p * rel_p).T @ np.abs(G) + group * product_bound(p.T, G)
+            for s in range(buckets):
+                z["dtable"][s, h] += ds[idx == s].sum()
+                e["dtable"][s, h] += e_ds[idx == s].sum() + 2 * (sk + 64) * U * np.abs(ds[idx == s]).sum()
+    return z, e

@@ -402,6 +402,206 @@ def test_distill_twice_is_the_same(hip, rng):
     assert np.array_equal(one[0][0], two[0][0]) and one[0][1] == two[0][1] and np.array_equal(one[2], two[2]) and np.array_equal(one[3], two[3])
 
 
+# ------------------------------------------------------------------ attention with a relative position bias
+
+def layout(a, order, pad=0, fill=np.nan):
+    """a [batch, heads, rows, d] in memory in the given order of the three, each row followed by `pad` floats; the array and
+    its (batch, head, row) strides in elements."""
+    t = np.transpose(a, [*order, 3])
+    p = np.full((*t.shape[:3], t.shape[3] + pad), fill, np.float32)
+    p[..., :t.shape[3]] = t
+    step = [p.shape[1] * p.shape[2] * p.shape[3], p.shape[2] * p.shape[3], p.shape[3]]
+    strides = [0, 0, 0]
+    for place, axis in enumerate(order):
+        strides[axis] = step[place]
+    return p, strides
+
+
+def unlayout(p, order, d):
+    back = [0, 0, 0]
+    for place, axis in enumerate(order):
+        back[axis] = place
+    return np.transpose(p[..., :d], [*back, 3])
+
+
+def run_attention(hip, q, k, v, table, lens, offset, buckets, distance, both, causal, scale, d_out=None, order=(0, 1, 2), pad=0, accumulate=None):
+    d = q.shape[3]
+    (pq, qs), (pk, ks), (pv, vs) = (layout(a, order, pad) for a in (q, k, v))
+    po, os_ = layout(np.full(q.shape, np.nan), order, pad, 7.0)
+    plan = hip.relbias_attention(batch=q.shape[0], heads=q.shape[1], kv_heads=k.shape[1], sq=q.shape[2], sk=k.shape[2], d=d, q_stride=qs,
+                                 k_stride=ks, v_stride=vs, o_stride=os_, query_offset=offset, num_buckets=buckets, max_distance=distance,
+                                 bidirectional=int(both), causal=int(causal), scale=scale)
+    dq, dk, dv, dt, dl, do = (dev(hip, x) for x in (pq, pk, pv, table, lens, po))
+    lse = dev(hip, np.full(q.shape[:3], np.nan, np.float32))
+    hip.check(hip.bh_relbias_attention_forward(plan, ptr(dq), ptr(dk), ptr(dv), ptr(dt), ptr(dl), ptr(do), ptr(lse)), "forward")
+    o = do.numpy()
+    assert pad == 0 or (o[..., d:] == 7.0).all()
+    got = {"out": unlayout(o, order, d), "lse": lse.numpy()}
+    if d_out is not None:
+        dd = dev(hip, layout(d_out, order, pad)[0])
+        gq, gk, gv = (dev(hip, np.full_like(x, 7.0)) for x in (pq, pk, pv))
+        gt = dev(hip, np.full(table.shape, np.nan, np.float32) if accumulate is None else accumulate)
+        hip.check(hip.bh_relbias_attention_backward(plan, ptr(dq), ptr(dk), ptr(dv), ptr(dt), ptr(dl), ptr(do), ptr(lse), ptr(dd), ptr(gq), ptr(gk),
+                                                    ptr(gv), ptr(gt), int(accumulate is not None)), "backward")
+        for n, x in (("dq", gq), ("dk", gk), ("dv", gv)):
+            x = x.numpy()
+            assert pad == 0 or (x[..., d:] == 7.0).all()
+            got[n] = unlayout(x, order, d)
+        got["dtable"] = gt.numpy()
+    return got
+
+
+def attention_case(rng, batch, heads, kv_heads, sq, sk, d, buckets):
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    return f(batch, heads, sq, d), f(batch, kv_heads, sk, d), f(batch, kv_heads, sk, d), f(buckets, heads), f(batch, heads, sq, d)
+
+
+def check_attention(hip, case, lens=None, offset=None, distance=20, both=False, causal=True, scale=None, train=True, order=(0, 1, 2), pad=0, poison=False):
+    q, k, v, table, d_out = case
+    offset = k.shape[2] - q.shape[2] if offset is None else offset
+    scale = q.shape[3] ** -0.5 if scale is None else scale
+    buckets = table.shape[0]
+    lens = None if lens is None else np.asarray(lens, np.int32)
+    want, bound = oc.attention(q, k, v, table, lens, offset, buckets, distance, both, causal, scale, d_out if train else None)
+    if poison:       # what lies behind a sequence is not read
+        for b, n in enumerate(lens):
+            k[b, :, max(int(n), 0):] = np.nan
+            v[b, :, max(int(n), 0):] = np.inf
+    got = run_attention(hip, q, k, v, table, lens, offset, buckets, distance, both, causal, scale, d_out if train else None, order, pad)
+    assert np.array_equal(np.isneginf(got["lse"]), np.isneginf(want["lse"]))
+    for n in got:
+        live = np.isfinite(want[n])
+        off = np.abs(got[n][live] - want[n][live]) / (bound[n][live] + 1e-37)
+        assert (off <= 1).all(), (n, off.max())
+    return got
+
+
+@pytest.mark.parametrize("rows", [0, 1])
+@pytest.mark.parametrize("d", [1, 8, 32, 33, 64, 80, 96, 100, 128])
+def test_attention_head_sizes(hip, rng, rows, d):
+    hip.check(hip.bh_relbias_attention_force_rows(rows))
+    try:
+        check_attention(hip, attention_case(rng, 2, 4, 2, 37, 70, d, 8), train=rows == 0)
+        check_attention(hip, attention_case(rng, 1, 2, 2, 130, 67, d, 12), both=True, causal=False, distance=40, train=rows == 0)
+    finally:
+        hip.check(hip.bh_relbias_attention_force_rows(-1))
+
+
+@pytest.mark.parametrize("rows", [0, 1])
+@pytest.mark.parametrize("sq,sk", [(1, 1), (1, 64), (1, 300), (2, 31), (31, 33), (32, 32), (33, 129), (64, 64), (65, 65), (128, 128), (129, 200), (200, 129),
+                                   (5, 0), (40, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_lengths(hip, rng, rows, sq, sk, causal):
+    hip.check(hip.bh_relbias_attention_force_rows(rows))
+    try:
+        check_attention(hip, attention_case(rng, 2, 2, 1, sq, sk, 32, 16), causal=causal, both=not causal, distance=50, train=rows == 0)
+    finally:
+        hip.check(hip.bh_relbias_attention_force_rows(-1))
+
+
+@pytest.mark.parametrize("rows", [0, 1])
+def test_attention_padded_batches(hip, rng, rows):
+    """Sequences of length zero, one, past a tile and beyond both ends; keys behind them hold NaN and infinities."""
+    hip.check(hip.bh_relbias_attention_force_rows(rows))
+    try:
+        for causal in (True, False):
+            got = check_attention(hip, attention_case(rng, 7, 2, 1, 45, 140, 40, 16), lens=[0, 1, 64, 65, 139, 500, -3], causal=causal, train=rows == 0,
+                                  poison=True)
+            assert (got["out"][0] == 0).all() and (got["out"][6] == 0).all()
+            if rows == 0:
+                assert (got["dk"][0] == 0).all() and (got["dv"][2, :, 64:] == 0).all() and (got["dq"][6] == 0).all()
+    finally:
+        hip.check(hip.bh_relbias_attention_force_rows(-1))
+
+
+@pytest.mark.parametrize("rows", [0, 1])
+@pytest.mark.parametrize("offset", [-60, -1, 0, 7, 300])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_offsets_and_rows_that_see_nothing(hip, rng, rows, offset, causal):
+    hip.check(hip.bh_relbias_attention_force_rows(rows))
+    try:
+        check_attention(hip, attention_case(rng, 1, 2, 2, 50, 90, 24, 32), offset=offset, causal=causal, both=True, distance=30, train=rows == 0)
+    finally:
+        hip.check(hip.bh_relbias_attention_force_rows(-1))
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2), (0, 2, 1), (2, 0, 1), (1, 0, 2)])
+@pytest.mark.parametrize("pad,d", [(0, 64), (4, 64), (3, 64), (1, 17)])
+def test_attention_layouts(hip, rng, order, pad, d):
+    check_attention(hip, attention_case(rng, 3, 4, 2, 70, 90, d, 16), lens=[90, 33, 70], order=order, pad=pad)
+    check_attention(hip, attention_case(rng, 2, 4, 4, 1, 90, d, 16), order=order, pad=pad, train=False)
+
+
+@pytest.mark.parametrize("buckets,distance,both", [(2, 2, False), (4, 3, True), (32, 128, True), (32, 128, False), (256, 1000, False), (256, 70, True)])
+def test_attention_buckets(hip, rng, buckets, distance, both):
+    for rows in (0, 1):
+        hip.check(hip.bh_relbias_attention_force_rows(rows))
+        try:
+            check_attention(hip, attention_case(rng, 1, 3, 3, 150, 330, 32, buckets), distance=distance, both=both, causal=False, train=rows == 0)
+        finally:
+            hip.check(hip.bh_relbias_attention_force_rows(-1))
+
+
+def test_attention_masked_buckets(hip, rng):
+    """-inf or the lowest float in the table masks its distances; a row with nothing else is empty."""
+    for low in (-np.inf, np.finfo(np.float32).min):
+        q, k, v, table, d_out = attention_case(rng, 1, 2, 2, 140, 140, 32, 8)
+        table[2:, 0] = low                     # head 0 sees the two nearest keys
+        table[:, 1] = low                      # head 1 nothing
+        got = check_attention(hip, (q, k, v, table, d_out))
+        assert (got["out"][0, 1] == 0).all() and np.isneginf(got["lse"][0, 1]).all()
+        assert (got["dq"][0, 1] == 0).all() and (got["dk"][0, 1] == 0).all() and (got["dtable"][:, 1] == 0).all()
+
+
+@pytest.mark.parametrize("sq,sk,rows", [(1, 5000, 1), (16, 3000, 1), (40, 2500, 0), (128, 1500, 0), (70, 4000, 1)])
+def test_attention_over_long_histories(hip, rng, sq, sk, rows):
+    hip.check(hip.bh_relbias_attention_force_rows(rows))
+    try:
+        check_attention(hip, attention_case(rng, 2, 2, 1, sq, sk, 64, 32), lens=[sk, sk // 3], distance=128, train=False)
+    finally:
+        hip.check(hip.bh_relbias_attention_force_rows(-1))
+
+
+def test_attention_training_of_a_longer_sequence(hip, rng):
+    check_attention(hip, attention_case(rng, 1, 2, 1, 600, 600, 64, 32), distance=128)
+    check_attention(hip, attention_case(rng, 1, 1, 1, 500, 700, 128, 64), both=True, causal=False, distance=1024)
+
+
+def test_attention_large_scores(hip, rng):
+    q, k, v, table, d_out = attention_case(rng, 1, 2, 2, 70, 100, 64, 16)
+    check_attention(hip, (q * 6, k * 6, v, table * 20, d_out), scale=0.3)
+    check_attention(hip, (q, k, v, table, d_out), scale=-1.0)
+    check_attention(hip, (q, k, v, table, d_out), scale=0.0)
+
+
+def test_attention_table_gradient_accumulates_and_repeats(hip, rng):
+    case = attention_case(rng, 2, 4, 2, 150, 150, 64, 16)
+    args = (*case[:4], None, 0, 16, 40, False, True, 0.125, case[4])
+    one, two = run_attention(hip, *args), run_attention(hip, *args)
+    for n in one:
+        assert np.array_equal(one[n], two[n])
+    start = rng.standard_normal(case[3].shape).astype(np.float32)
+    more = run_attention(hip, *args, accumulate=start)
+    assert (np.abs(more["dtable"] - (start.astype(np.float64) + one["dtable"])) <= 2 * oc.U * (np.abs(start) + np.abs(one["dtable"]))).all()
+
+
+def test_attention_against_differences(hip, rng):
+    q, k, v, table, d_out = attention_case(rng, 1, 2, 1, 20, 24, 8, 8)
+    args = (None, 4, 8, 12, False, True, 0.4)
+    got = run_attention(hip, q, k, v, table, *args, d_out)
+
+    def loss(*x):
+        return float((oc.attention(*x, *args)[0]["out"] * d_out).sum())
+    eps = 1e-5
+    for at, n in enumerate(("dq", "dk", "dv", "dtable")):
+        base = [x.astype(np.float64) for x in (q, k, v, table)]
+        d = rng.standard_normal(base[at].shape)
+        up, down = list(base), list(base)
+        up[at], down[at] = base[at] + eps * d, base[at] - eps * d
+        # third derivatives of order ten times eps^2, 1e-16 |loss| / eps, and fp32 gradients
+        assert abs(float((got[n] * d).sum()) - (loss(*up) - loss(*down)) / (2 * eps)) <= 1e-5 * float(np.abs(got[n] * d).sum() + 1)
+
+
 # ------------------------------------------------------------------ all of them
 
 def test_capture_is_refused(hip):
@@ -410,14 +610,17 @@ def test_capture_is_refused(hip):
     graph = C.c_void_p()
     d = dev(hip, np.ones(64, np.float32))
     i = dev(hip, np.zeros(64, np.int32))
+    plan = hip.relbias_attention(batch=1, heads=1, kv_heads=1, sq=2, sk=2, d=4, q_stride=(8, 8, 4), k_stride=(8, 8, 4), v_stride=(8, 8, 4),
+                                 o_stride=(8, 8, 4), query_offset=0, num_buckets=4, max_distance=8, bidirectional=0, causal=0, scale=1.0)
     assert rt.hipStreamBeginCapture(C.c_void_p(hip.bh_stream()), 2) == 0
     try:
         rcs = [hip.bh_gemm_epilogue(0, 0, 4, 4, 4, ptr(d), 4, ptr(d), 4, ptr(d, 32), 4, None, -1, None, 0, None, 0),
-               hip.bh_distill_forward(ptr(d), 8, ptr(d), ptr(i), None, 2, 8, 2, 1.0, 1.0, 1.0, None, None, ptr(d, 32))]
+               hip.bh_distill_forward(ptr(d), 8, ptr(d), ptr(i), None, 2, 8, 2, 1.0, 1.0, 1.0, None, None, ptr(d, 32)),
+               hip.bh_relbias_attention_forward(plan, ptr(d), ptr(d), ptr(d), ptr(d), None, ptr(d, 32), ptr(d, 48))]
         text = hip.bh_last_error().decode()
     finally:
         assert rt.hipStreamEndCapture(C.c_void_p(hip.bh_stream()), C.byref(graph)) == 0
         if graph:
             rt.hipGraphDestroy(graph)
-    assert rcs == [-1, -1] and "captured" in text
+    assert rcs == [-1, -1, -1] and "captured" in text
     assert (d.numpy() == 1).all()

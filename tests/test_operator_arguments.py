@@ -68,3 +68,63 @@ def test_distillation_gradient_refusals():
     refused(hip.bh_distill_loss_grad(*distill_args(), None, None, ANY, 101), "in place")
     refused(hip.bh_distill_backward(*distill_args(), None, None, C.c_void_p(128), 100), "null")
     refused(hip.bh_distill_backward(*distill_args(), ANY, None, ANY, 101), "in place")
+
+
+# ------------------------------------------------------------------ attention with a relative position bias
+
+@pytest.mark.parametrize("buckets,distance,both", [(32, 128, 1), (32, 128, 0), (2, 2, 0), (4, 5, 1), (3, 9, 0), (48, 250, 1), (64, 1024, 0), (256, 100000, 0),
+                                                   (256, 129, 0), (16, 64, 1)])
+def test_buckets_against_whole_numbers(buckets, distance, both):
+    import operator_cases as oc
+    for r in list(range(-300, 301)) + [-distance, distance, -distance - 1, distance - 1, 1 - distance, 10 ** 12, -10 ** 12]:
+        assert hip.bh_relative_position_bucket(r, buckets, distance, both) == oc.bucket(r, buckets, distance, both), r
+
+
+@pytest.mark.parametrize("buckets,distance,both", [(1, 10, 0), (0, 10, 0), (257, 1000, 0), (5, 100, 1), (2, 100, 1), (32, 16, 0), (32, 8, 1), (32, -1, 0)])
+def test_bucket_refusals(buckets, distance, both):
+    assert hip.bh_relative_position_bucket(3, buckets, distance, both) == -1
+    assert "buckets" in hip.bh_last_error().decode()
+
+
+def description(**change):
+    a = dict(batch=2, heads=4, kv_heads=2, sq=3, sk=5, d=8, q_stride=(96, 24, 8), k_stride=(80, 40, 8), v_stride=(80, 40, 8), o_stride=(96, 24, 8),
+             query_offset=2, num_buckets=8, max_distance=20, bidirectional=0, causal=1, scale=1.0)
+    a.update(change)
+    return hip.relbias_attention(**a)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(batch=-1), "negative"), (dict(sq=-1), "negative"), (dict(sk=-1), "negative"), (dict(d=0), "head size"), (dict(d=129), "head size"),
+    (dict(kv_heads=3), "multiple"), (dict(kv_heads=0), "multiple"), (dict(sk=1 << 29), "2^28"), (dict(query_offset=-(1 << 29)), "2^28"),
+    (dict(q_stride=(96, -24, 8)), "negative stride"), (dict(num_buckets=1), "buckets"), (dict(max_distance=4), "buckets"),
+    (dict(bidirectional=1, num_buckets=7), "buckets"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(batch=1 << 20, heads=1 << 12, kv_heads=1), "heads"),
+])
+def test_attention_refusals(change, text):
+    p = description(**change)
+    refused(hip.bh_relbias_attention_forward(p, ANY, ANY, ANY, ANY, None, ANY, ANY), text)
+    refused(hip.bh_relbias_attention_backward(p, ANY, ANY, ANY, ANY, None, ANY, ANY, ANY, ANY, ANY, ANY, ANY, 0), text)
+
+
+def test_attention_pointer_and_overlap_refusals():
+    p = description()
+    for at in (0, 1, 2, 3, 5, 6):
+        args = [ANY] * 7
+        args[at] = None
+        refused(hip.bh_relbias_attention_forward(p, *args), "null")
+    for at in (0, 1, 2, 3, 5, 6, 7, 8, 9, 10, 11):
+        args = [ANY] * 12
+        args[at] = None
+        refused(hip.bh_relbias_attention_backward(p, *args, 0), "null")
+    refused(hip.bh_relbias_attention_forward(None, *[ANY] * 7), "null")
+    refused(hip.bh_relbias_attention_forward(description(o_stride=(96, 24, 7)), *[ANY] * 7), "overlap")
+    refused(hip.bh_relbias_attention_forward(description(o_stride=(0, 24, 8)), *[ANY] * 7), "overlap")
+    # a key that several sequences share (a stride of zero) can be read, but its gradient has no place
+    refused(hip.bh_relbias_attention_backward(description(k_stride=(0, 40, 8)), *[ANY] * 12, 0), "overlap")
+    refused(hip.bh_relbias_attention_backward(description(sq=0), *[ANY] * 12, 0), "without queries")
+
+
+def test_empty_attention_needs_no_device():
+    for change in (dict(batch=0), dict(sq=0), dict(heads=0)):
+        assert hip.bh_relbias_attention_forward(description(**change), *[None] * 7) == 0
+    assert hip.bh_relbias_attention_backward(description(batch=0), *[None] * 12, 0) == 0
