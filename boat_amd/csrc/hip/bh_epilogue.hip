@@ -11,6 +11,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace bh {
 
 struct EpiArgs {
@@ -141,7 +143,7 @@ __device__ __forceinline__ void finish_block(const EpiArgs& g, const f32x16 (&ac
 // KC: the contraction index is the fast one in memory (a thread takes 8 consecutive floats of one row, its neighbour the other
 // half: the padding keeps the two halves' writes in different banks); otherwise the output index is (a thread takes 8 floats
 // down one column).
-template <bool KC, int R, int NT>
+template <bool KC, bool VEC, int R, int NT>
 struct SplitOperand {
     static constexpr int KG = 16 * R + 64;
     static constexpr int PLANE = 2 * KG;
@@ -150,53 +152,70 @@ struct SplitOperand {
     static_assert(2 * R % NT == 0, "whole units per thread");
 
     float reg[PER][8];
+    // the next step's place: an address that is the same for the wavefront and an offset per unit that never changes
+    const float* base[PER];
+    unsigned off[PER];
+    int64_t step;
 
     static __device__ __forceinline__ void unit(int tid, int i, int& row, int& kg) {
         const int u = tid + i * NT;
-        if (KC) { row = u >> 1; kg = u & 1; } else { row = u % R; kg = u / R; }
+        if (KC) { row = u >> 1; kg = u & 1; } else { row = u % R; kg = __builtin_amdgcn_readfirstlane(u / R); }
     }
-    // rows past the matrix are clamped (their products are not stored), the tail of the contraction is zero
-    __device__ __forceinline__ void load(const float* __restrict__ p, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int64_t k1,
-                                         bool vec, int tid) {
+    // rows past the matrix are clamped: their products are not stored
+    __device__ __forceinline__ void init(const float* __restrict__ p, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int tid) {
+        step = KC ? 16 : 16 * ld;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             int row, kg;
             unit(tid, i, row, kg);
-            int64_t r = row0 + row;
-            if (r >= rows) r = rows - 1;
-            const int64_t k = k0 + 8 * kg;
-            if (k0 + 16 <= k1) {
-                if (KC) {
-                    const float* q = p + r * ld + k;
-                    if (vec) {
-                        const f32x4 x = *reinterpret_cast<const f32x4*>(q), y = *reinterpret_cast<const f32x4*>(q + 4);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) { reg[i][e] = x[e]; reg[i][4 + e] = y[e]; }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; e++) reg[i][e] = q[e];
-                    }
-                } else {
-                    const float* q = p + k * ld + r;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) reg[i][e] = q[e * ld];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) reg[i][e] = k + e < k1 ? (KC ? p[r * ld + k + e] : p[(k + e) * ld + r]) : 0.f;
-            }
+            const unsigned r = (unsigned)(min(row0 + row, rows - 1) - row0);
+            base[i] = KC ? p + row0 * ld + k0 : p + (k0 + 8 * kg) * ld + row0;
+            off[i] = KC ? 4u * (r * (unsigned)ld + 8u * kg) : 4u * r;
         }
     }
-    __device__ __forceinline__ void store(char* lds, int tid) const {
+    static __device__ __forceinline__ const float* place(const float* b, unsigned o) {
+        return reinterpret_cast<const float*>(reinterpret_cast<const char*>(b) + o);
+    }
+    // unit i of 16 of the contraction that are all there
+    __device__ __forceinline__ void load(int i, int64_t ld) {
+        if (KC && VEC) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(place(base[i], off[i])), y = *reinterpret_cast<const f32x4*>(place(base[i] + 4, off[i]));
+#pragma unroll
+            for (int e = 0; e < 4; e++) { reg[i][e] = x[e]; reg[i][4 + e] = y[e]; }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) reg[i][e] = *place(base[i] + (KC ? e : e * ld), off[i]);
+        }
+        base[i] += step;
+    }
+    // the last ones: `left` (1 to 15) are there, the others count as zero
+    __device__ __forceinline__ void load_tail(int64_t ld, int left, int tid) {
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             int row, kg;
             unit(tid, i, row, kg);
-            u32x4 p[kPlanes];
-            split_eight(reg[i], p);
+#pragma unroll
+            for (int e = 0; e < 8; e++) reg[i][e] = 8 * kg + e < left ? *place(base[i] + (KC ? e : e * ld), off[i]) : 0.f;
+        }
+    }
+    // two of unit i's eight floats; with the last two the unit's pieces go to LDS
+    __device__ __forceinline__ void split_part(int i, int part, u32x4 (&p)[kPlanes], char* lds, int tid) const {
+        unsigned h, m, l;
+        split_pair(reg[i][2 * part], reg[i][2 * part + 1], h, m, l);
+        p[0][part] = h; p[1][part] = m; p[2][part] = l;
+        if (part == 3) {
+            int row, kg;
+            unit(tid, i, row, kg);
 #pragma unroll
             for (int q = 0; q < kPlanes; q++) *reinterpret_cast<u32x4*>(lds + q * PLANE + kg * KG + row * 16) = p[q];
         }
+    }
+    __device__ __forceinline__ void store(char* lds, int tid) const {
+        u32x4 p[kPlanes];
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+#pragma unroll
+            for (int part = 0; part < 4; part++) split_part(i, part, p, lds, tid);
     }
     // rows 32*b .. 32*b + 31
     static __device__ __forceinline__ void fragment(const char* lds, int b, int lane, u32x4 (&f)[kPlanes]) {
@@ -216,16 +235,17 @@ typedef SplitTile<2, 2, 2, 2, 2> Tile128;
 
 template <typename Cfg, bool A_KC, bool B_KC>
 struct TileLds {
-    static constexpr int STAGE = SplitOperand<A_KC, Cfg::BM, Cfg::NT>::BYTES + SplitOperand<B_KC, Cfg::BN, Cfg::NT>::BYTES;
+    static constexpr int STAGE = SplitOperand<A_KC, true, Cfg::BM, Cfg::NT>::BYTES + SplitOperand<B_KC, true, Cfg::BN, Cfg::NT>::BYTES;
     static constexpr int EPI = Cfg::WM * Cfg::WN * EpiBlock<Cfg::TN>::BYTES;
     static constexpr int BYTES = 2 * STAGE > EPI ? 2 * STAGE : EPI;
 };
 
-template <typename Cfg, bool A_KC, bool B_KC>
-__global__ __launch_bounds__(Cfg::NT, Cfg::WGS) void epilogue_tile_kernel(EpiArgs g, bool vec_a, bool vec_b, bool vec_c) {
+// VEC: the operands whose contraction index is the fast one can be read 16 bytes at a time
+template <typename Cfg, bool A_KC, bool B_KC, bool VEC>
+__global__ __launch_bounds__(Cfg::NT, Cfg::WGS) void epilogue_tile_kernel(EpiArgs g, bool vec_c) {
     constexpr int TM = Cfg::TM, TN = Cfg::TN;
-    using OpA = SplitOperand<A_KC, Cfg::BM, Cfg::NT>;
-    using OpB = SplitOperand<B_KC, Cfg::BN, Cfg::NT>;
+    using OpA = SplitOperand<A_KC, VEC, Cfg::BM, Cfg::NT>;
+    using OpB = SplitOperand<B_KC, VEC, Cfg::BN, Cfg::NT>;
     constexpr int STAGE = TileLds<Cfg, A_KC, B_KC>::STAGE;
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -234,7 +254,8 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::WGS) void epilogue_tile_kernel(EpiArg
     tile_of(blockIdx.x, g.tiles_m, g.tiles_n, tm, tn);
     const int64_t m0 = (int64_t)tm * Cfg::BM, n0 = (int64_t)tn * Cfg::BN;
     const int64_t kb = blockIdx.y * g.k_per_split, ke = min(g.k, kb + g.k_per_split);
-    const int steps = ke > kb ? (int)((ke - kb + 15) / 16) : 0;
+    const int whole = ke > kb ? (int)((ke - kb) / 16) : 0, left = ke > kb ? (int)((ke - kb) % 16) : 0;
+    const int steps = whole + (left ? 1 : 0);
 
     f32x16 acc[TM][TN];
 #pragma unroll
@@ -246,35 +267,67 @@ __global__ __launch_bounds__(Cfg::NT, Cfg::WGS) void epilogue_tile_kernel(EpiArg
 
     OpA oa;
     OpB ob;
+    oa.init(g.a, g.lda, m0, g.m, kb, tid);
+    ob.init(g.b, g.ldb, n0, g.n, kb, tid);
     const auto fetch = [&](int s) {
-        oa.load(g.a, g.lda, m0, g.m, kb + 16 * s, ke, vec_a, tid);
-        ob.load(g.b, g.ldb, n0, g.n, kb + 16 * s, ke, vec_b, tid);
+        if (s < whole) {
+#pragma unroll
+            for (int i = 0; i < OpA::PER; i++) oa.load(i, g.lda);
+#pragma unroll
+            for (int i = 0; i < OpB::PER; i++) ob.load(i, g.ldb);
+        } else if (s < steps) {
+            oa.load_tail(g.lda, left, tid);
+            ob.load_tail(g.ldb, left, tid);
+        }
+    };
+    const auto put = [&](int s) {
+        oa.store(smem + (s & 1) * STAGE, tid);
+        ob.store(smem + (s & 1) * STAGE + OpA::BYTES, tid);
+    };
+    // A step's products, and between the 32 x 32 tiles' a share of the splitting of the next step's operands (in registers since
+    // the step before) and of the loads of the one after: what a wavefront issues while the matrix core is busy costs nothing.
+    const auto step = [&](int s, auto more) {
+        const char* cur = smem + (s & 1) * STAGE;
+        char* next = smem + (s & 1 ^ 1) * STAGE;
+        u32x4 fa[2][kPlanes], fb[TN][kPlanes], planes[kPlanes];
+        OpB::fragment(cur + OpA::BYTES, wn * TN, lane, fb[0]);
+        OpA::fragment(cur, wm * TM, lane, fa[0]);
+#pragma unroll
+        for (int j = 1; j < TN; j++) OpB::fragment(cur + OpA::BYTES, wn * TN + j, lane, fb[j]);
+        constexpr int PARTS = 4 * (OpA::PER + OpB::PER), TILES = TM * TN;
+#pragma unroll
+        for (int t = 0; t < TILES; t++) {
+            const int i = t / TN, j = t % TN;
+            if (j == 0 && i + 1 < TM) OpA::fragment(cur, wm * TM + i + 1, lane, fa[(i + 1) & 1]);
+            acc[i][j] = mfma_split(fa[i & 1], fb[j], acc[i][j]);
+            if constexpr (decltype(more)::value) {
+#pragma unroll
+                for (int x = t * PARTS / TILES; x < (t + 1) * PARTS / TILES; x++) {
+                    if (x < 4 * OpA::PER) {
+                        oa.split_part(x / 4, x % 4, planes, next, tid);
+                        if (x % 4 == 3) oa.load(x / 4, g.lda);
+                    } else {
+                        ob.split_part(x / 4 - OpA::PER, x % 4, planes, next + OpA::BYTES, tid);
+                        if (x % 4 == 3) ob.load(x / 4 - OpA::PER, g.ldb);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        __syncthreads();
     };
     if (steps > 0) {
         fetch(0);
-        oa.store(smem, tid);
-        ob.store(smem + OpA::BYTES, tid);
-        if (steps > 1) fetch(1);
+        put(0);
+        fetch(1);
     }
     __syncthreads();
-    for (int s = 0; s < steps; s++) {
-        const char* cur = smem + (s & 1) * STAGE;
-        char* next = smem + ((s & 1) ^ 1) * STAGE;
-        u32x4 fa[TM][kPlanes], fb[TN][kPlanes];
-#pragma unroll
-        for (int i = 0; i < TM; i++) OpA::fragment(cur, wm * TM + i, lane, fa[i]);
-#pragma unroll
-        for (int j = 0; j < TN; j++) OpB::fragment(cur + OpA::BYTES, wn * TN + j, lane, fb[j]);
-        if (s + 1 < steps) {                     // the other stage is free since the last barrier
-            oa.store(next, tid);
-            ob.store(next + OpA::BYTES, tid);
-        }
-        if (s + 2 < steps) fetch(s + 2);
-#pragma unroll
-        for (int i = 0; i < TM; i++)
-#pragma unroll
-            for (int j = 0; j < TN; j++) acc[i][j] = mfma_split(fa[i], fb[j], acc[i][j]);
-        __syncthreads();
+    int s = 0;
+    for (; s + 2 < whole; s++) step(s, std::true_type{});
+    for (; s < steps; s++) {                     // the last two or three: what is left to load and to split
+        if (s + 1 < steps) put(s + 1);
+        fetch(s + 2);
+        step(s, std::false_type{});
     }
 
     const int64_t row0 = m0 + wm * 32 * TM, col0 = n0 + wn * 32 * TN;
@@ -341,51 +394,79 @@ __device__ __forceinline__ void direct_fragment(const float* __restrict__ p, int
     }
 }
 
-constexpr int kSmallWaves = 8;
-template <bool A_KC, bool B_KC>
-__global__ __launch_bounds__(64 * kSmallWaves) void epilogue_small_kernel(EpiArgs g, bool vec_a, bool vec_b) {
-    __shared__ float sums[kSmallWaves][32 * 33];
+template <int T_, int WAVES_>
+struct SmallTile {
+    static constexpr int T = T_, WAVES = WAVES_, SIZE = 32 * T, NT = 64 * WAVES;   // T x T blocks of 32 x 32
+};
+typedef SmallTile<1, 8> Small32;
+typedef SmallTile<2, 8> Small64;
+typedef SmallTile<1, 16> SmallLong;
+
+template <typename Cfg, bool A_KC, bool B_KC>
+__global__ __launch_bounds__(Cfg::NT) void epilogue_small_kernel(EpiArgs g, bool vec_a, bool vec_b) {
+    constexpr int T = Cfg::T, WAVES = Cfg::WAVES;
+    __shared__ float sums[WAVES][32 * 33];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t m0 = (int64_t)(blockIdx.x / g.tiles_n) * 32, n0 = (int64_t)(blockIdx.x % g.tiles_n) * 32;
+    const int64_t m0 = (int64_t)(blockIdx.x / g.tiles_n) * Cfg::SIZE, n0 = (int64_t)(blockIdx.x % g.tiles_n) * Cfg::SIZE;
     const int64_t kb = blockIdx.y * g.k_per_split, ke = min(g.k, kb + g.k_per_split);
-    const int64_t row = min(m0 + (lane & 31), g.m - 1), col = min(n0 + (lane & 31), g.n - 1);
-    f32x16 acc;
+    int64_t row[T], col[T];                      // past the matrix the last one is read, its products are not stored
 #pragma unroll
-    for (int e = 0; e < 16; e++) acc[e] = 0.f;
+    for (int i = 0; i < T; i++) {
+        row[i] = min(m0 + 32 * i + (lane & 31), g.m - 1);
+        col[i] = min(n0 + 32 * i + (lane & 31), g.n - 1);
+    }
+    f32x16 acc[T][T];
+#pragma unroll
+    for (int i = 0; i < T; i++)
+#pragma unroll
+        for (int j = 0; j < T; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
     // kDepth steps' loads are issued before the first one's products
-    constexpr int kDepth = 2, kStep = 16 * kSmallWaves;
+    constexpr int kDepth = T == 1 && WAVES == 8 ? 2 : 1, kStep = 16 * WAVES;
     const int64_t half = 8 * (lane >> 5);
     for (int64_t k = kb + 16 * wave; k < ke; k += kDepth * kStep) {
-        float x[kDepth][8], y[kDepth][8];
+        float x[kDepth][T][8], y[kDepth][T][8];
+#pragma unroll
+        for (int d = 0; d < kDepth; d++)
+#pragma unroll
+            for (int i = 0; i < T; i++) {
+                direct_fragment<A_KC>(g.a, g.lda, row[i], k + d * kStep + half, ke, vec_a, x[d][i]);
+                direct_fragment<B_KC>(g.b, g.ldb, col[i], k + d * kStep + half, ke, vec_b, y[d][i]);
+            }
 #pragma unroll
         for (int d = 0; d < kDepth; d++) {
-            direct_fragment<A_KC>(g.a, g.lda, row, k + d * kStep + half, ke, vec_a, x[d]);
-            direct_fragment<B_KC>(g.b, g.ldb, col, k + d * kStep + half, ke, vec_b, y[d]);
-        }
+            u32x4 fa[T][kPlanes], fb[T][kPlanes];
 #pragma unroll
-        for (int d = 0; d < kDepth; d++) {
-            u32x4 fa[kPlanes], fb[kPlanes];
-            split_eight(x[d], fa);
-            split_eight(y[d], fb);
-            acc = mfma_split(fa, fb, acc);
+            for (int i = 0; i < T; i++) { split_eight(x[d][i], fa[i]); split_eight(y[d][i], fb[i]); }
+#pragma unroll
+            for (int i = 0; i < T; i++)
+#pragma unroll
+                for (int j = 0; j < T; j++) acc[i][j] = mfma_split(fa[i], fb[j], acc[i][j]);
         }
     }
 #pragma unroll
-    for (int e = 0; e < 16; e++) sums[wave][acc_row(e, lane) * 33 + (lane & 31)] = acc[e];
-    __syncthreads();
-    for (int i = tid; i < 32 * 32; i += 64 * kSmallWaves) {
-        const int64_t r = m0 + (i >> 5), c = n0 + (i & 31);
-        if (r >= g.m || c >= g.n) continue;
-        float s = 0.f;
+    for (int i = 0; i < T; i++)
 #pragma unroll
-        for (int w = 0; w < kSmallWaves; w++) s += sums[w][(i >> 5) * 33 + (i & 31)];
-        if (g.splits > 1) {
-            g.partial[((int64_t)blockIdx.y * g.m + r) * g.n + c] = s;
-        } else {
-            if (!finite_f32(s)) s = plain_element<A_KC, B_KC>(g, r, c, 0, g.k);
-            finish_element(g, r, c, s);
+        for (int j = 0; j < T; j++) {
+            if (i + j > 0) __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 16; e++) sums[wave][acc_row(e, lane) * 33 + (lane & 31)] = acc[i][j][e];
+            __syncthreads();
+            for (int q = tid; q < 32 * 32; q += Cfg::NT) {
+                const int64_t r = m0 + 32 * i + (q >> 5), c = n0 + 32 * j + (q & 31);
+                if (r >= g.m || c >= g.n) continue;
+                float s = 0.f;
+#pragma unroll
+                for (int w = 0; w < WAVES; w++) s += sums[w][(q >> 5) * 33 + (q & 31)];
+                if (g.splits > 1) {
+                    g.partial[((int64_t)blockIdx.y * g.m + r) * g.n + c] = s;
+                } else {
+                    if (!finite_f32(s)) s = plain_element<A_KC, B_KC>(g, r, c, 0, g.k);
+                    finish_element(g, r, c, s);
+                }
+            }
         }
-    }
 }
 
 // ---------------------------------------------------------------------------------------------------- choice and launch
@@ -393,31 +474,44 @@ static int g_force_variant = -1, g_force_splits = 0;
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <typename Cfg, bool A_KC, bool B_KC>
-static int launch_tile(const EpiArgs& g, bool va, bool vb, bool vc) {
+template <typename Cfg, bool A_KC, bool B_KC, bool VEC>
+static int launch_tile(const EpiArgs& g, bool vc) {
     constexpr int bytes = TileLds<Cfg, A_KC, B_KC>::BYTES;
     static bool raised = false;                 // more than 64 KB of LDS has to be asked for once
     if (!raised) {
-        const int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(&epilogue_tile_kernel<Cfg, A_KC, B_KC>),
+        const int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(&epilogue_tile_kernel<Cfg, A_KC, B_KC, VEC>),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "bh_gemm_epilogue: LDS size");
         if (rc) return rc;
         raised = true;
     }
-    hipLaunchKernelGGL((epilogue_tile_kernel<Cfg, A_KC, B_KC>), dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(Cfg::NT),
-                       bytes, stream(), g, va, vb, vc);
+    hipLaunchKernelGGL((epilogue_tile_kernel<Cfg, A_KC, B_KC, VEC>), dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(Cfg::NT),
+                       bytes, stream(), g, vc);
     return BH_LAUNCH_CHECK("bh_gemm_epilogue");
 }
+template <typename Cfg, bool A_KC, bool B_KC>
+static int launch_tile(const EpiArgs& g, bool va, bool vb, bool vc) {
+    if constexpr (A_KC || B_KC)
+        if ((A_KC && !va) || (B_KC && !vb)) return launch_tile<Cfg, A_KC, B_KC, false>(g, vc);
+    return launch_tile<Cfg, A_KC, B_KC, true>(g, vc);
+}
 
-enum { kTile256 = 0, kTile128 = 1, kSmall = 2 };
+enum { kTile256 = 0, kTile128, kSmall32, kSmall64, kSmallLong, kVariants };
+struct TileSize { int m, n; };
+static const TileSize kSizes[kVariants] = {{Tile256::BM, Tile256::BN}, {Tile128::BM, Tile128::BN}, {32, 32}, {64, 64}, {32, 32}};
+
+template <typename Cfg, bool A_KC, bool B_KC>
+static int launch_small(const EpiArgs& g, bool va, bool vb) {
+    hipLaunchKernelGGL((epilogue_small_kernel<Cfg, A_KC, B_KC>), dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(Cfg::NT), 0,
+                       stream(), g, va, vb);
+    return BH_LAUNCH_CHECK("bh_gemm_epilogue");
+}
 
 template <bool A_KC, bool B_KC>
 static int run_product(EpiArgs g, int variant, int splits) {
     const bool va = A_KC && g.lda % 4 == 0 && aligned16(g.a), vb = B_KC && g.ldb % 4 == 0 && aligned16(g.b);
     const bool vc = g.ldc % 4 == 0 && aligned16(g.c) && (!g.saved || (g.lds % 4 == 0 && aligned16(g.saved))) &&
                     (!g.residual || (g.ldr % 4 == 0 && aligned16(g.residual)));
-    const int bm = variant == kTile256 ? Tile256::BM : variant == kTile128 ? Tile128::BM : 32;
-    const int bn = variant == kTile256 ? Tile256::BN : variant == kTile128 ? Tile128::BN : 32;
-    const int64_t tiles_m = ceil_div(g.m, bm), tiles_n = ceil_div(g.n, bn);
+    const int64_t tiles_m = ceil_div(g.m, kSizes[variant].m), tiles_n = ceil_div(g.n, kSizes[variant].n);
     if (tiles_m * tiles_n > 0x7fffffff) return set_error(BH_EINVAL, "bh_gemm_epilogue: output too large");
     g.tiles_m = (int)tiles_m;
     g.tiles_n = (int)tiles_n;
@@ -431,21 +525,66 @@ static int run_product(EpiArgs g, int variant, int splits) {
     int rc;
     if (variant == kTile256) rc = launch_tile<Tile256, A_KC, B_KC>(g, va, vb, vc);
     else if (variant == kTile128) rc = launch_tile<Tile128, A_KC, B_KC>(g, va, vb, vc);
-    else {
-        hipLaunchKernelGGL((epilogue_small_kernel<A_KC, B_KC>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)g.splits), dim3(64 * kSmallWaves), 0,
-                           stream(), g, va, vb);
-        rc = BH_LAUNCH_CHECK("bh_gemm_epilogue");
-    }
+    else if (variant == kSmall64) rc = launch_small<Small64, A_KC, B_KC>(g, va, vb);
+    else if (variant == kSmallLong) rc = launch_small<SmallLong, A_KC, B_KC>(g, va, vb);
+    else rc = launch_small<Small32, A_KC, B_KC>(g, va, vb);
     if (rc || g.splits == 1) return rc;
     const int64_t blocks = ceil_div(g.m * g.n, 256);
     hipLaunchKernelGGL((epilogue_fold_kernel<A_KC, B_KC>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream(), g);
     return BH_LAUNCH_CHECK("bh_gemm_epilogue: fold");
 }
 
+// What a variant is expected to take, in us, so that the fastest is chosen.  A workgroup's steps (16 of the contraction; a small
+// tile's wavefronts take that many each) last `alone` where it has the compute unit to itself, and `shared` times the workgroups
+// on the unit where they fill it; each output tile costs `finish`, the launch `fixed`, and an operand that is read along its
+// rows makes the steps `rows` longer.  A cut contraction adds a launch and its partial sums' traffic.  Fitted to 520 shapes of
+// 1 to 8192 rows and 60 to 4100 features, all variants and cuts, three layouts: the choice is 2 % over the best one in the
+// mean, 8 % at most for nine shapes in ten.
+struct Cost { float alone, shared, finish, fixed, rows; int per_cu, waves; };
+static const Cost kCost[kVariants] = {
+    {2.05f, 2.05f, 9.65f, 4.67f, 0.f, 1, 1},       // 256 x 256
+    {0.74f, 0.641f, 1.58f, 7.85f, 0.f, 3, 1},      // 128 x 128
+    {0.015f, 0.609f, 1.11f, 2.20f, 0.232f, 2, 8},  // 32 x 32
+    {1.76f, 1.37f, 4.17f, 0.56f, 0.073f, 1, 8},    // 64 x 64, wavefronts cut the contraction
+    {1.19f, 0.501f, 1.12f, 1.11f, 0.125f, 1, 16},  // 32 x 32, twice the wavefronts
+};
+static double cost_of(int variant, int64_t m, int64_t n, int64_t k, int splits, int along_rows) {
+    const Cost& c = kCost[variant];
+    const int64_t per_split = ceil_div(ceil_div(k, splits), 16) * 16;
+    const double cuts = (double)ceil_div(k, per_split);
+    const double wgs = (double)ceil_div(m, kSizes[variant].m) * (double)ceil_div(n, kSizes[variant].n) * cuts;
+    const double steps = (double)ceil_div(per_split, 16 * c.waves), slow = 1.0 + c.rows * along_rows;
+    const double full = floor(wgs / (256.0 * c.per_cu)), rest = ceil((wgs - full * 256.0 * c.per_cu) / 256.0);
+    double t = c.fixed;
+    if (full > 0) t += full * (steps * slow * fmax(c.alone, c.per_cu * c.shared) + c.per_cu * c.finish);
+    if (rest > 0) t += steps * slow * fmax(c.alone, rest * c.shared) + rest * c.finish;
+    if (cuts > 1) t += 3.2 + 1.07e-6 * cuts * (double)m * (double)n;
+    return t;
+}
+static void choose(int64_t m, int64_t n, int64_t k, int along_rows, int& variant, int& splits) {
+    static const int kCuts[] = {1, 2, 3, 4, 6, 8, 12, 16, 32};
+    double best = 1e30;
+    variant = kSmall32;
+    splits = 1;
+    for (int v = 0; v < kVariants; v++) {
+        const double flops = 2.0 * (double)m * (double)n * (double)k;
+        if ((v == kSmallLong && k < 256) || ((v == kSmall32 || v == kSmallLong) && flops > 2e10) || (v == kSmall64 && flops > 1e11)) continue;
+        const int64_t tiles = ceil_div(m, kSizes[v].m) * ceil_div(n, kSizes[v].n);
+        for (int s : kCuts) {
+            if (s > 1 && (k / s < 64 || tiles * s > 2048 || (double)s * m * n > 1.3e8)) break;
+            const double t = cost_of(v, m, n, k > 0 ? k : 1, s, along_rows);
+            if (t < best) { best = t; variant = v; splits = s; }
+        }
+    }
+}
+
 static int product(int trans_a, int trans_b, EpiArgs g) {
-    int variant = g.m * g.n >= 128 * 128 * 64 ? kTile128 : kSmall, splits = 1;
-    if (g_force_variant >= 0) variant = g_force_variant;
+    constexpr int64_t kMaxLd = (int64_t)1 << 22;   // 256 rows of a tile within 32 bits of bytes; past it the small tiles' addresses
+    int variant, splits;
+    choose(g.m, g.n, g.k, (trans_a ? 1 : 0) + (trans_b ? 0 : 1), variant, splits);
+    if (g_force_variant >= 0) { variant = g_force_variant; splits = 1; }
     if (g_force_splits > 0) splits = g_force_splits;
+    if (variant <= kTile128 && (g.lda >= kMaxLd || g.ldb >= kMaxLd)) { variant = kSmall64; splits = 1; }
     if (!trans_a) return trans_b ? run_product<true, true>(g, variant, splits) : run_product<true, false>(g, variant, splits);
     return trans_b ? run_product<false, true>(g, variant, splits) : run_product<false, false>(g, variant, splits);
 }
@@ -501,7 +640,7 @@ int bh_dense_act_backward(int act, const float* x, const float* w, const float* 
 }
 
 int bh_gemm_epilogue_force(int variant, int splits) {
-    BH_CHECK_ARG(variant >= -1 && variant <= 2 && splits >= 0 && splits <= 64, "variant -1 to 2, 0 to 64 splits");
+    BH_CHECK_ARG(variant >= -1 && variant < kVariants && splits >= 0 && splits <= 64, "variant -1 to 4, 0 to 64 splits");
     g_force_variant = variant;
     g_force_splits = splits;
     return BH_OK;

@@ -404,8 +404,8 @@ int bh_gemm_no_tables(int off);
 int bh_sdpa_force_general(int on);
 /* bh_relbias_attention_force_rows: 1 = the forward pass's kernel for few query rows, 0 = its tiles, -1 = by shape (default) */
 int bh_relbias_attention_force_rows(int mode);
-/* bh_gemm_epilogue_force: variant 0 = 256x256, 1 = 128x128 tiles, 2 = 32x32 (small problems), -1 = by shape (default);
- * splits > 0: cut the contraction this many ways, 0 = by shape */
+/* bh_gemm_epilogue_force: variant 0 = 256x256, 1 = 128x128 tiles through LDS, 2 = 32x32, 3 = 64x64, 4 = 32x32 with sixteen
+ * wavefronts (small problems), -1 = by shape (default); splits > 0: cut the contraction this many ways, 0 = by shape */
 int bh_gemm_epilogue_force(int variant, int splits);
 /* bh_sdpa_force_wide: 1 = the attention backward's 256-key workgroups (eight wavefronts) wherever that form exists
  * (head_dim 32 and 64), 0 = never, -1 = chosen by shape (the default) */

@@ -78,7 +78,7 @@ def check_product(hip, rng, m, n, k, ta, tb, act, with_bias, with_residual, keep
         assert rel_fro(y, want) <= fp32_gemm_bound(k)    # what narrower operands would fail
 
 
-@pytest.mark.parametrize("variant", [0, 1, 2])
+@pytest.mark.parametrize("variant", [0, 1, 2, 3, 4])
 @pytest.mark.parametrize("ta,tb", [(0, 0), (0, 1), (1, 0), (1, 1)])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (33, 31, 17), (129, 257, 100), (256, 128, 64), (300, 140, 523)])
 def test_product_every_tile(hip, rng, variant, ta, tb, m, n, k):
@@ -91,7 +91,7 @@ def test_product_every_tile(hip, rng, variant, ta, tb, m, n, k):
 
 
 @pytest.mark.parametrize("act", list(oc.ACTS))
-@pytest.mark.parametrize("variant", [0, 1, 2])
+@pytest.mark.parametrize("variant", [0, 1, 2, 3, 4])
 def test_product_activations(hip, rng, act, variant):
     hip.check(hip.bh_gemm_epilogue_force(variant, 0))
     try:
@@ -101,7 +101,7 @@ def test_product_activations(hip, rng, act, variant):
         hip.check(hip.bh_gemm_epilogue_force(-1, 0))
 
 
-@pytest.mark.parametrize("variant,splits", [(0, 2), (0, 7), (1, 3), (2, 2), (2, 64)])
+@pytest.mark.parametrize("variant,splits", [(0, 2), (0, 7), (1, 3), (2, 2), (2, 64), (3, 3), (4, 2)])
 @pytest.mark.parametrize("ta,tb", [(0, 0), (0, 1), (1, 0), (1, 1)])
 def test_product_split_contraction(hip, rng, variant, splits, ta, tb):
     hip.check(hip.bh_gemm_epilogue_force(variant, splits))
@@ -128,7 +128,7 @@ def test_product_without_contraction_and_without_rows(hip, rng):
     assert (d.numpy() == 3.0).all()
 
 
-@pytest.mark.parametrize("variant,splits", [(0, 0), (1, 0), (2, 0), (1, 3)])
+@pytest.mark.parametrize("variant,splits", [(0, 0), (1, 0), (2, 0), (1, 3), (3, 0), (4, 2)])
 def test_product_infinities_and_nan(hip, rng, variant, splits):
     """What is not finite comes out as fp32 arithmetic gives it; the other rows and columns are untouched by it."""
     hip.check(hip.bh_gemm_epilogue_force(variant, splits))
