@@ -49,10 +49,11 @@ struct RelArgs {
     int splits; int64_t keys_per_split;    // forward over few workgroups: partial results per split
     float *part_o, *part_ml;               // [split][batch*heads*sq][d], [split][batch*heads*sq][2]
     float* delta;                          // backward: rowsum(dO o O)
-    float* part_table;                     // backward: [batch*heads][query tiles][buckets]
+    double* part_table;                    // backward: [batch*heads][query tiles][buckets]
     int buckets, q_tiles;
     const char *k_row, *k_col, *v_row, *v_col, *q_row, *q_col, *g_row, *g_col;   // planes
     int k_blocks, q_blocks;                // of 32 rows, per head
+    float *part_k, *part_v;                // backward, shared key heads: [batch*heads][sk][d]
     Buckets b;
 };
 
@@ -595,8 +596,8 @@ template <int DP> struct QueryLds {
     static constexpr int BORDER = 3 * Block<DP>::BYTES;
     static constexpr int VALUE = BORDER + 4 * (kMaxBuckets / 2 + 4);
     static constexpr int WIN = VALUE + 4 * kMaxBuckets;
-    static constexpr int SUMS = WIN + kWaves * 64 * 4;                        // per wavefront: a sum per bucket
-    static constexpr int BLOCK = SUMS + kWaves * kMaxBuckets * 4;             // per wavefront: a block of dS, rows of 33
+    static constexpr int SUMS = WIN + kWaves * 64 * 4;                        // per wavefront: a sum per bucket, in 64 bits
+    static constexpr int BLOCK = SUMS + kWaves * kMaxBuckets * 8;             // per wavefront: a block of dS, rows of 33
     static constexpr int BYTES = BLOCK + kWaves * 32 * 33 * 4;
 };
 
@@ -610,7 +611,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
     float* value = reinterpret_cast<float*>(smem + L::VALUE);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     float* win = reinterpret_cast<float*>(smem + L::WIN) + 64 * wave;
-    float* sums = reinterpret_cast<float*>(smem + L::SUMS) + kMaxBuckets * wave;
+    double* sums = reinterpret_cast<double*>(smem + L::SUMS) + kMaxBuckets * wave;
     float* block = reinterpret_cast<float*>(smem + L::BLOCK) + 32 * 33 * wave;
     int bh, tile;
     head_and_tile(blockIdx.x, g.batch * g.heads, g.q_tiles, bh, tile);
@@ -619,7 +620,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
     const float* dout = g.d_out + bt * g.os[0] + h * g.os[1];
     const int64_t plane0 = ((int64_t)bt * g.kv_heads + hk) * g.k_blocks * Block<DP>::BYTES;
     stage_bias(g, h, border, value, kThreads);
-    for (int i = lane; i < g.buckets; i += 64) sums[i] = 0.f;
+    for (int i = lane; i < g.buckets; i += 64) sums[i] = 0.0;
     const Bias bias = {border, value};
 
     const int q0 = tile * kQueryTile, qw = q0 + 32 * wave, qi = qw + (lane & 31);
@@ -634,23 +635,32 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
         copy_to_lds<KB, kWaves>(g.v_row + at, smem + L::V, wave, lane);
     };
     if (ke > 0) fetch_rows(0);
+    // The matrix cores' sums are cut towards minus infinity by some hundredths of a step.  For one element that is nothing, but
+    // the table's gradient adds up a million of them that nearly cancel: odd queries are negated, and their results again, so
+    // that the cuts cancel too (8 x 16 heads x 1024 x 1024: the table's relative error 4e-6 without, 4e-7 with it).
+    const float sign = lane & 1 ? -1.f : 1.f;
     u32x4 qf[KD][kPlanes], gf[KD][kPlanes];
     const int64_t qrow = min((int64_t)qi, g.sq - 1);
 #pragma unroll
     for (int s = 0; s < KD; s++) {
         float x[8];
         row_eight(q + qrow * g.qs[2], live, 16 * s + 8 * (lane >> 5), g.d, g.vec_q, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] *= sign;
         split_eight(x, qf[s]);
         row_eight(dout + qrow * g.os[2], live, 16 * s + 8 * (lane >> 5), g.d, g.vec_o, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] *= sign;
         split_eight(x, gf[s]);
     }
     const int64_t row = (int64_t)bh * g.sq + qrow;
     const float lse = lse_log2(g.lse_in[row]), delta = g.delta[row];
-    const float c = g.scale * kLog2e;
+    const float c = g.scale * kLog2e * sign;
     f32x16 dq[ND];
 #pragma unroll
     for (int b = 0; b < ND; b++) dq[b] = zero16();
-    float far_sum[2] = {0.f, 0.f};                                            // blocks that lie in one bucket: before, behind
+    // A bucket's sum is small against its terms (a row of dS adds up to zero): blocks are added up in 64 bits
+    double far_sum[2] = {0.0, 0.0};                                           // blocks that lie in one bucket: before, behind
     wait_copies();
     for (int k0 = 0; k0 < ke; k0 += KEYS) {
         copy_to_lds<KB, kWaves>(g.k_col + plane0 + (int64_t)(k0 / 32) * Block<DP>::BYTES, smem + L::KT, wave, lane);
@@ -671,12 +681,13 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
         int bucket = 0, constant;
         finish_scores(g, bias, s, c, k0 - rel_q, ke - k0, win, lane, bucket, constant);
 #pragma unroll
-        for (int e = 0; e < 16; e++) s[e] = live ? __builtin_amdgcn_exp2f(s[e] - lse) * (dp[e] - delta) : 0.f;
+        for (int e = 0; e < 16; e++) s[e] = live ? __builtin_amdgcn_exp2f(s[e] - lse) * fmaf(dp[e], sign, -delta) : 0.f;
         if (constant >= 0) {
-            float t = 0.f;
+            float t[8];
 #pragma unroll
-            for (int e = 0; e < 16; e++) t += s[e];
-            if (constant == g.b.side - 1) far_sum[0] += t; else far_sum[1] += t;
+            for (int e = 0; e < 8; e++) t[e] = s[e] + s[8 + e];
+            const double all = (double)((t[0] + t[1]) + (t[2] + t[3])) + (double)((t[4] + t[5]) + (t[6] + t[7]));
+            if (constant == g.b.side - 1) far_sum[0] += all; else far_sum[1] += all;
         } else {
             // diagonal `lane` of the block: key row r, query column x with r - x = lane - 31
             __builtin_amdgcn_wave_barrier();
@@ -685,22 +696,27 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            float t = 0.f;
-#pragma unroll 8
-            for (int x = 0; x < 32; x++) {
-                const int r = lane - 31 + x;
-                const float y = block[min(max(r, 0), 31) * 33 + x];
-                t += r >= 0 && r < 32 ? y : 0.f;
+            double t = 0.0;
+#pragma unroll 2
+            for (int x0 = 0; x0 < 32; x0 += 8) {
+                float part[8];
+#pragma unroll
+                for (int x = 0; x < 8; x++) {
+                    const int r = lane - 31 + x0 + x;
+                    const float y = block[min(max(r, 0), 31) * 33 + x0 + x];
+                    part[x] = r >= 0 && r < 32 ? y : 0.f;
+                }
+                t += (double)((part[0] + part[1]) + (part[2] + part[3])) + (double)((part[4] + part[5]) + (part[6] + part[7]));
             }
             // lanes of one bucket are neighbours: sums of runs, the last lane of a run adds it to the bucket
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) {
-                const float y = __shfl_up(t, off, 64);
+                const double y = __shfl_up(t, off, 64);
                 const int other = __shfl_up(bucket, off, 64);
                 if (lane >= off && other == bucket) t += y;
             }
-            const int next = __shfl_down(bucket, 1, 64);
-            if (lane == 63 || next != bucket) sums[bucket] += t;
+            const int after = __shfl_down(bucket, 1, 64);
+            if (lane == 63 || after != bucket) sums[bucket] += t;
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
@@ -713,14 +729,14 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
         }
         wait_copies();
     }
-    far_sum[0] = wave_sum(far_sum[0]);
-    far_sum[1] = wave_sum(far_sum[1]);
+    far_sum[0] = wave_sum_f64(far_sum[0]);
+    far_sum[1] = wave_sum_f64(far_sum[1]);
     if (lane == 0) {
         sums[g.b.side - 1] += far_sum[0];
         sums[g.b.both ? 2 * g.b.side - 1 : 0] += far_sum[1];
     }
     __syncthreads();
-    const float* all = reinterpret_cast<const float*>(smem + L::SUMS);
+    const double* all = reinterpret_cast<const double*>(smem + L::SUMS);
     for (int i = tid; i < g.buckets; i += kThreads)
         g.part_table[((int64_t)bh * g.q_tiles + tile) * g.buckets + i] =
             (all[i] + all[kMaxBuckets + i]) + (all[2 * kMaxBuckets + i] + all[3 * kMaxBuckets + i]);
@@ -751,7 +767,7 @@ __global__ __launch_bounds__(256) void relattn_table_kernel(RelArgs g, float* __
     if (b < g.buckets)
         for (int i = part; i < total; i += 16) {
             const int64_t bh = (int64_t)(i / g.q_tiles) * g.heads + h;
-            s += (double)g.part_table[(bh * g.q_tiles + i % g.q_tiles) * g.buckets + b];
+            s += g.part_table[(bh * g.q_tiles + i % g.q_tiles) * g.buckets + b];
         }
     red[threadIdx.x] = s;
     __syncthreads();
@@ -773,7 +789,8 @@ template <int DP> struct KeyLds {
     static constexpr int BYTES = WIN + kWaves * 64 * 4;
 };
 
-// dK and dV: a workgroup owns 128 keys of a key head and walks over the queries of all heads that share it
+// dK and dV of one query head: a workgroup owns 128 keys and walks over the queries.  Heads that share a key head leave their
+// parts in work memory (one long chain of sums over all of them would round more, and fill fewer compute units)
 template <int DP>
 __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel(RelArgs g, int k_tiles) {
     using L = KeyLds<DP>;
@@ -784,9 +801,9 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     float* win = reinterpret_cast<float*>(smem + L::WIN) + 64 * wave;
     int bh, tile;
-    head_and_tile(blockIdx.x, g.batch * g.kv_heads, k_tiles, bh, tile);
+    head_and_tile(blockIdx.x, g.batch * g.heads, k_tiles, bh, tile);
     tile = k_tiles - 1 - tile;                                                // the first keys are seen by the most queries
-    const int bt = bh / g.kv_heads, hk = bh % g.kv_heads;
+    const int bt = bh / g.heads, h = bh % g.heads, hk = h / g.group;
     const float* k = g.k + bt * g.ks[0] + hk * g.ks[1];
     const float* v = g.v + bt * g.vs[0] + hk * g.vs[1];
     const int kw = tile * 128 + 32 * wave, ki = kw + (lane & 31), sq = (int)g.sq;
@@ -808,10 +825,12 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
     int qb = 0;                                                               // causal: the first query that sees a key of the workgroup
     if (g.causal) qb = (int)(min((int64_t)sq, max((int64_t)0, (int64_t)tile * 128 - g.offset)) / ROWS * ROWS);
     if (tile * 128 >= len) qb = sq;                                           // only padding here
-    for (int hg = 0; hg < g.group && qb < sq; hg++) {
-        const int h = hk * g.group + hg;
-        const int64_t row0 = ((int64_t)bt * g.heads + h) * g.sq;
-        const int64_t plane0 = ((int64_t)bt * g.heads + h) * g.q_blocks * Block<DP>::BYTES;
+    // One turn of a loop that the compiler cannot see to be one: it then keeps the fragments' making apart from the steps.
+    // Run together they need 47 registers more than there are at head size 128.
+    int turns = 1;
+    asm volatile("" : "+s"(turns));
+    for (; turns > 0 && qb < sq; turns--) {
+        const int64_t row0 = (int64_t)bh * g.sq, plane0 = (int64_t)bh * g.q_blocks * Block<DP>::BYTES;
         const auto fetch = [&](const char* q, const char* d, int r0, int at) {
             const int64_t o = plane0 + (int64_t)(r0 / 32) * Block<DP>::BYTES;
             copy_to_lds<KB, kWaves>(q + o, smem + at, wave, lane);
@@ -823,7 +842,6 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
                 reinterpret_cast<float*>(smem + L::STAT)[64 * buffer + tid] = tid < ROWS ? lse_log2(g.lse_in[row0 + r]) : g.delta[row0 + r];
             }
         };
-        // the heads before are done with LDS: their loop ends behind a barrier
         stage_bias(g, h, border, value, kThreads);
         const Bias bias = {border, value};
         fetch(g.q_row, g.g_row, qb, 0);
@@ -891,27 +909,44 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
         }
     }
     if (ki >= g.sk) return;
-    float* pk = g.dk + bt * g.ks[0] + hk * g.ks[1] + ki * g.ks[2];
-    float* pv = g.dv + bt * g.vs[0] + hk * g.vs[1] + ki * g.vs[2];
+    const bool shared = g.group > 1;
+    const int64_t at = ((int64_t)bh * g.sk + ki) * g.d;
+    float* pk = shared ? g.part_k + at : g.dk + bt * g.ks[0] + hk * g.ks[1] + ki * g.ks[2];
+    float* pv = shared ? g.part_v + at : g.dv + bt * g.vs[0] + hk * g.vs[1] + ki * g.vs[2];
+    const bool vec_k = shared ? g.d % 4 == 0 : g.vec_k, vec_v = shared ? g.d % 4 == 0 : g.vec_v;
 #pragma unroll
-    for (int b = 0; b < DP / 32; b++)
+    for (int b = 0; b < ND; b++)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
             const int cd = 32 * b + acc_row(e, lane);
             f32x4 x, y;
 #pragma unroll
             for (int j = 0; j < 4; j++) { x[j] = dk[b][e + j] * g.scale; y[j] = dv[b][e + j]; }
-            if (g.vec_k && cd + 4 <= g.d) *reinterpret_cast<f32x4*>(pk + cd) = x;
+            if (vec_k && cd + 4 <= g.d) *reinterpret_cast<f32x4*>(pk + cd) = x;
             else
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     if (cd + j < g.d) pk[cd + j] = x[j];
-            if (g.vec_v && cd + 4 <= g.d) *reinterpret_cast<f32x4*>(pv + cd) = y;
+            if (vec_v && cd + 4 <= g.d) *reinterpret_cast<f32x4*>(pv + cd) = y;
             else
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     if (cd + j < g.d) pv[cd + j] = y[j];
+            __builtin_amdgcn_sched_barrier(0);
         }
+}
+
+// the parts of the heads that share a key head, in order
+__global__ __launch_bounds__(256) void relattn_heads_kernel(RelArgs g) {
+    const int64_t per = g.sk * g.d, total = (int64_t)g.batch * g.kv_heads * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t bk = i / per, at = i - bk * per, row = at / g.d, c = at - row * g.d, bt = bk / g.kv_heads, hk = bk - bt * g.kv_heads;
+        const int64_t first = (bt * g.heads + hk * g.group) * per + at;
+        float x = g.part_k[first], y = g.part_v[first];
+        for (int h = 1; h < g.group; h++) { x += g.part_k[first + h * per]; y += g.part_v[first + h * per]; }
+        g.dk[bt * g.ks[0] + hk * g.ks[1] + row * g.ks[2] + c] = x;
+        g.dv[bt * g.vs[0] + hk * g.vs[1] + row * g.vs[2] + c] = y;
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------- host side
@@ -1079,9 +1114,9 @@ static int run_backward(RelArgs& g, float* dtable, int accumulate) {
     static bool raised_q = false, raised_k = false;
     const int64_t rows = (int64_t)g.batch * g.heads * g.sq, wgs = (int64_t)g.q_tiles * g.batch * g.heads;
     Scratch delta, table, planes;
-    if (!delta.get(sizeof(float) * (size_t)rows) || !table.get(sizeof(float) * (size_t)wgs * (size_t)g.buckets)) return BH_ENOMEM;
+    if (!delta.get(sizeof(float) * (size_t)rows) || !table.get(sizeof(double) * (size_t)wgs * (size_t)g.buckets)) return BH_ENOMEM;
     g.delta = (float*)delta.p;
-    g.part_table = (float*)table.p;
+    g.part_table = (double*)table.p;
     hipLaunchKernelGGL(relattn_delta_kernel, dim3((unsigned)ceil_div(rows, 16)), dim3(256), 0, stream(), g);
     int rc = BH_LAUNCH_CHECK("bh_relbias_attention_backward: delta");
     if (rc) return rc;
@@ -1111,10 +1146,21 @@ static int run_backward(RelArgs& g, float* dtable, int accumulate) {
         if (rc) return rc;
         raised_k = true;
     }
+    Scratch heads;
+    if (g.group > 1) {
+        const size_t each = (size_t)g.batch * g.heads * (size_t)g.sk * g.d;
+        if (!heads.get(2 * sizeof(float) * each)) return BH_ENOMEM;
+        g.part_k = (float*)heads.p;
+        g.part_v = g.part_k + each;
+    }
     const int k_tiles = (int)ceil_div(g.sk, 128);
-    hipLaunchKernelGGL(relattn_dkv_kernel<DP>, dim3((unsigned)((int64_t)k_tiles * g.batch * g.kv_heads)), dim3(kThreads), KeyLds<DP>::BYTES, stream(),
+    hipLaunchKernelGGL(relattn_dkv_kernel<DP>, dim3((unsigned)((int64_t)k_tiles * g.batch * g.heads)), dim3(kThreads), KeyLds<DP>::BYTES, stream(),
                        g, k_tiles);
-    return BH_LAUNCH_CHECK("bh_relbias_attention_backward: dk, dv");
+    rc = BH_LAUNCH_CHECK("bh_relbias_attention_backward: dk, dv");
+    if (rc || g.group == 1) return rc;
+    const int64_t blocks = ceil_div((int64_t)g.batch * g.kv_heads * g.sk * g.d, 256);
+    hipLaunchKernelGGL(relattn_heads_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream(), g);
+    return BH_LAUNCH_CHECK("bh_relbias_attention_backward: heads");
 }
 
 }  // namespace bh
