@@ -17,12 +17,14 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace bh {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // rows of odd length start anywhere
 
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kMaxTopk = 4096;
 
 struct DistillArgs {
@@ -31,6 +33,7 @@ struct DistillArgs {
     const int32_t* labels;                         // [rows] or NULL
     int64_t rows; int vocab; int topk;
     float cold;                                    // log2(e) / T
+    int power;                                     // T where it is 1, 2, 3 or 4, else 0: exp(x) is then exp(x/T)^T
     float inv_t, w_soft, w_hard;                   // 1/T, alpha T^2, 1 - alpha (0 without labels)
     float g_soft, g_hard;                          // scale alpha T, scale (1 - alpha)
     const float* seed;                             // device scalar on the gradient, or NULL
@@ -54,29 +57,44 @@ struct RowStats {
     }
 };
 
+// The exponents are fma(z, log2(e)/T, -max log2(e)/T), one rounding each; the rounding of the second product is the same factor
+// in every term and in the sum.  Where T is a small whole number the softmax at 1 takes its terms from the one at T: the
+// exponential is the slowest instruction here (a quarter of the rate of the others).
+template <int POWER>
+__device__ __forceinline__ float hard_term(float soft, float z, float off) {
+    if (POWER == 1) return soft;
+    if (POWER == 2) return soft * soft;
+    if (POWER == 3) return soft * soft * soft;
+    if (POWER == 4) return (soft * soft) * (soft * soft);
+    return fast_exp2(fmaf(z, kLog2e, off));
+}
+template <int POWER, bool HARD, int N>
+__device__ __forceinline__ void add_terms(const f32x4 (&v)[N], float b, float cold, float& a, float& c) {
+    const float off = -b * cold, off1 = -b * kLog2e;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const float t = fast_exp2(fmaf(v[i][q], cold, off));
+            a += t;
+            if (HARD) c += hard_term<POWER>(t, v[i][q], off1);
+        }
+        __builtin_amdgcn_sched_barrier(0);   // one vector's temporaries at a time: the registers hold the row
+    }
+}
 template <int N>
-__device__ __forceinline__ void stats_of(const f32x4 (&v)[N], float cold, bool hard, RowStats& s) {
+__device__ __forceinline__ void stats_of(const f32x4 (&v)[N], float cold, bool hard, int power, RowStats& s) {
     float top = s.m;
 #pragma unroll
     for (int i = 0; i < N; i++) top = fmaxf(fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3])), top);
     const float b = RowStats::base(top);
     float a = s.st * fast_exp2((s.m - b) * cold), c = s.s1 * fast_exp2((s.m - b) * kLog2e);
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-#pragma unroll
-        for (int q = 0; q < 4; q++) a += fast_exp2((v[i][q] - b) * cold);
-        __builtin_amdgcn_sched_barrier(0);   // one vector's temporaries at a time: the registers hold the row
-    }
-    if (hard) {
-        float again = b;                     // ... and the differences are taken anew
-        asm volatile("" : "+v"(again));
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-#pragma unroll
-            for (int q = 0; q < 4; q++) c += fast_exp2((v[i][q] - again) * kLog2e);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
+    if (!hard) add_terms<0, false>(v, b, cold, a, c);
+    else if (power == 1) add_terms<1, true>(v, b, cold, a, c);
+    else if (power == 2) add_terms<2, true>(v, b, cold, a, c);
+    else if (power == 3) add_terms<3, true>(v, b, cold, a, c);
+    else if (power == 4) add_terms<4, true>(v, b, cold, a, c);
+    else add_terms<0, true>(v, b, cold, a, c);
     s.m = top; s.st = a; s.s1 = c;
 }
 
@@ -96,21 +114,32 @@ __device__ __forceinline__ RowStats block_stats(RowStats s, float cold, float (*
     return t;
 }
 
-// A part [begin, end) of a row: vectors of four from begin on, and up to three elements behind them, one to a thread.
-// Loads past the last vector read the last one and count as -inf, so that no branch stands between a thread's loads.
+// A part [begin, end) of a row: up to three elements, vectors of four from the first 16-byte boundary on, up to three elements
+// behind them (rows of odd length start anywhere; vectors across the boundaries cost 10 %).  The single elements are one to a
+// thread.  Loads past the last vector read the last one and count as -inf, so that no branch stands between a thread's loads.
 struct Span {
     const float* z;
-    int vecs, tail;            // whole vectors; elements behind them
-    __device__ __forceinline__ Span(const float* row, int begin, int end) : z(row + begin), vecs((end - begin) >> 2), tail((end - begin) & 3) {}
+    int head, vecs, tail;      // elements before the vectors; whole vectors; elements behind
+    __device__ __forceinline__ Span(const float* row, int begin, int end) {
+        const int n = end - begin;
+        head = min((int)((16 - (reinterpret_cast<uintptr_t>(row + begin) & 15)) & 15) >> 2, n);
+        vecs = (n - head) >> 2;
+        tail = (n - head) & 3;
+        z = row + begin + head;
+    }
+    template <bool ONCE = false>   // ONCE: not read again, does not stay in the caches
     __device__ __forceinline__ f32x4 load(int i) const {
         f32x4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         if (vecs > 0) {        // the same for the whole launch
-            const f32x4 u = *reinterpret_cast<const f32x4u*>(z + 4 * (unsigned)min(i, vecs - 1));
+            const f32x4u* p = reinterpret_cast<const f32x4u*>(z + 4 * (unsigned)min(i, vecs - 1));
+            const f32x4 u = ONCE ? __builtin_nontemporal_load(p) : *p;
             if (i < vecs) v = u;
         }
         return v;
     }
-    __device__ __forceinline__ float rest(int tid) const { return tid < tail ? z[4 * vecs + tid] : -INFINITY; }
+    __device__ __forceinline__ bool single(int tid) const { return tid < head + tail; }
+    __device__ __forceinline__ int place(int tid) const { return tid < head ? tid - head : 4 * vecs + tid - head; }   // from z
+    __device__ __forceinline__ float rest(int tid) const { return single(tid) ? z[place(tid)] : -INFINITY; }
 };
 __device__ __forceinline__ void stats_of_one(float x, float cold, RowStats& s) {
     s.join(RowStats{x, x == -INFINITY ? 0.f : 1.f, x == -INFINITY ? 0.f : 1.f}, cold);
@@ -122,26 +151,30 @@ struct Entries {
     float* value;     // [topk + 1] teacher logit / T
     float* logit;     // [topk + 1] student logit at the index
 };
-__device__ __forceinline__ Entries entries_at(float* lds, int n) { return {reinterpret_cast<int*>(lds), lds + n, lds + 2 * n}; }
+// the indices come first and fill whole vectors of four (-2 behind the label)
+__host__ __device__ __forceinline__ int entry_slots(int topk) { return (topk + 1 + 3) / 4 * 4; }
+__device__ __forceinline__ Entries entries_at(float* lds, int slots) { return {reinterpret_cast<int*>(lds), lds + slots, lds + 2 * slots}; }
 
-__device__ __forceinline__ void stage_entries(const DistillArgs& g, int64_t row, const Entries& e, const float* z, const float* gathered,
-                                              int threads) {
-    for (int j = threadIdx.x; j <= g.topk; j += threads) {
-        int i = -1;
-        float t = -INFINITY, x = 0.f;
+// entry j of a row as memory has it
+struct Entry {
+    int index;
+    float value;
+    __device__ __forceinline__ Entry(const DistillArgs& g, int64_t row, int j) : index(j > g.topk ? -2 : -1), value(-INFINITY) {
         if (j < g.topk) {
-            i = g.index[row * g.topk + j];
-            t = g.teacher[row * g.topk + j] * g.inv_t;
-        } else if (g.labels) {
-            i = g.labels[row];
+            index = g.index[row * g.topk + j];
+            value = g.teacher[row * g.topk + j] * g.inv_t;
+        } else if (j == g.topk && g.labels) {
+            index = g.labels[row];
         }
-        if (i < 0 || i >= g.vocab) i = -1;
-        if (i < 0) t = -INFINITY; else x = gathered ? gathered[row * (g.topk + 1) + j] : z[i];
-        e.index[j] = i;
-        e.value[j] = t;
-        e.logit[j] = x;
     }
-}
+    // z: the row's logits; only those in [begin, end) are looked at
+    __device__ __forceinline__ void stage(const DistillArgs& g, const Entries& e, int j, const float* z, int begin, int end) {
+        if (j <= g.topk && (index < 0 || index >= g.vocab)) index = -1;
+        e.index[j] = index;
+        e.value[j] = index < 0 ? -INFINITY : value;
+        e.logit[j] = index >= begin && index < end ? z[index] : 0.f;
+    }
+};
 // maximum and sum of the teacher's softmax, by every wavefront on its own
 __device__ __forceinline__ void teacher_softmax(const DistillArgs& g, const Entries& e, float& top, float& inv_sum) {
     const int lane = threadIdx.x & 63;
@@ -165,31 +198,73 @@ __device__ __forceinline__ float row_loss_of(const DistillArgs& g, const Entries
         const float ls = logf(sum), lt = logf(s.st), inv = 1.f / sum;
         for (int j = lane; j < g.topk; j += 64) {
             const float lp = e.value[j] - top, p = fast_exp2(lp * kLog2e) * inv;
-            if (p > 0.f || p != p) acc += p * ((lp - ls) - ((e.logit[j] - b) * g.inv_t - lt));
+            if (p > 0.f || p != p) acc += p * ((lp - ls) - (fmaf(e.logit[j], g.cold, -b * g.cold) * kLn2 - lt));
         }
     }
     acc = wave_sum(acc) * g.w_soft;
-    if (g.w_hard != 0.f && e.index[g.topk] >= 0) acc += g.w_hard * (logf(s.s1) - (e.logit[g.topk] - b));
+    if (g.w_hard != 0.f && e.index[g.topk] >= 0) acc += g.w_hard * (logf(s.s1) - fmaf(e.logit[g.topk], kLog2e, -b * kLog2e) * kLn2);
     return acc;
 }
 
-struct GradRow { float base, cold, ct, c1; };   // dz = ct exp2((z - base) cold) + c1 exp2((z - base) log2 e)
+// a row's loss and statistics, by its first wavefront
+__device__ __forceinline__ void finish_row(const DistillArgs& g, const Entries& e, const RowStats& s, float top, float sum, int64_t row) {
+    const float l = row_loss_of(g, e, s, top, sum);
+    if (threadIdx.x == 0) {
+        g.row_loss[row] = l;
+        if (g.stats) { g.stats[3 * row] = s.m; g.stats[3 * row + 1] = s.st; g.stats[3 * row + 2] = s.s1; }
+    }
+}
+// loss = scale * sum of the rows' losses, in a fixed order.  (A count of finished rows, whose last one adds them up in the same
+// launch, costs more than this launch: 96 rows of 1000 logits 9.8 us against 9.2, 1024 rows 32 against 10.5.)
+__global__ __launch_bounds__(1024) void distill_loss_kernel(const float* __restrict__ row_loss, int64_t rows, float scale, float* out) {
+    __shared__ double red[16];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < rows; i += 1024) s += (double)row_loss[i];
+    s = wave_sum_f64(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int i = 0; i < 16; i++) t += red[i];
+        out[0] = (float)(t * (double)scale);
+    }
+}
+
+struct GradRow { float cold, off, off1, ct, c1; int power; };   // dz = ct exp2(z cold + off) + c1 exp2(z log2 e + off1)
 
 __device__ __forceinline__ GradRow grad_row(const DistillArgs& g, const Entries& e, const RowStats& s, float sum) {
-    const float seed = g.seed ? g.seed[0] : 1.f;
-    return {RowStats::base(s.m), g.cold, sum != 0.f ? g.g_soft * seed / s.st : 0.f,
-            g.w_hard != 0.f && e.index[g.topk] >= 0 ? g.g_hard * seed / s.s1 : 0.f};
+    const float seed = g.seed ? g.seed[0] : 1.f, b = RowStats::base(s.m);
+    const bool hard = g.w_hard != 0.f && e.index[g.topk] >= 0;
+    return {g.cold, -b * g.cold, -b * kLog2e, sum != 0.f ? g.g_soft * seed / s.st : 0.f, hard ? g.g_hard * seed / s.s1 : 0.f, g.power};
 }
-__device__ __forceinline__ float grad_at(const GradRow& r, float z) {
-    float d = r.ct == 0.f ? 0.f : r.ct * fast_exp2((z - r.base) * r.cold);
-    if (r.c1 != 0.f) d += r.c1 * fast_exp2((z - r.base) * kLog2e);
+// POWER as above; -1: without the softmax at 1
+template <int POWER>
+__device__ __forceinline__ float grad_term(const GradRow& r, float z) {
+    const float t = fast_exp2(fmaf(z, r.cold, r.off)), d = r.ct * t;
+    return POWER < 0 ? d : fmaf(r.c1, hard_term<POWER>(t, z, r.off1), d);
+}
+// calls f with the power as a constant: which it is holds for the whole launch, so the choice stands outside the loops
+template <typename F>
+__device__ __forceinline__ void with_power(bool hard, int power, F f) {
+    if (!hard) f(std::integral_constant<int, -1>{});
+    else if (power == 1) f(std::integral_constant<int, 1>{});
+    else if (power == 2) f(std::integral_constant<int, 2>{});
+    else if (power == 3) f(std::integral_constant<int, 3>{});
+    else if (power == 4) f(std::integral_constant<int, 4>{});
+    else f(std::integral_constant<int, 0>{});
+}
+__device__ __forceinline__ float grad_at(const GradRow& r, bool hard, float z) {
+    float d = 0.f;
+    with_power(hard, r.power, [&](auto p) { d = grad_term<decltype(p)::value>(r, z); });
     return d;
 }
+// the gradient is not read again here: its stores pass the caches by, which keep the logits (131072 logits: 476 us against 571)
+template <int POWER>
 __device__ __forceinline__ void grad_store(const GradRow& r, f32x4 v, float* __restrict__ dz, int i, int vecs) {
     f32x4 d;
 #pragma unroll
-    for (int q = 0; q < 4; q++) d[q] = grad_at(r, v[q]);
-    if (i < vecs) *reinterpret_cast<f32x4u*>(dz + 4 * (unsigned)i) = d;
+    for (int q = 0; q < 4; q++) d[q] = grad_term<POWER>(r, v[q]);
+    if (i < vecs) __builtin_nontemporal_store(d, reinterpret_cast<f32x4u*>(dz + 4 * (unsigned)i));
 }
 // the places of [begin, end) that the teacher or the label names, behind the dense stores
 __device__ __forceinline__ void grad_entries(const DistillArgs& g, const Entries& e, const GradRow& r, float top, float sum, float* dz,
@@ -199,78 +274,111 @@ __device__ __forceinline__ void grad_entries(const DistillArgs& g, const Entries
     for (int j = threadIdx.x; j <= g.topk; j += threads) {
         const int i = e.index[j];
         if (i < begin || i >= end) continue;
-        bool first = true;
-        float w = 0.f;
-        for (int o = 0; o <= g.topk; o++) {
-            if (e.index[o] != i) continue;
-            if (o < j) { first = false; break; }
-            w += o == g.topk ? hard : soft == 0.f ? 0.f : soft * fast_exp2((e.value[o] - top) * kLog2e);
+        // how often does the index occur?  Mostly once; else the first entry takes the weights of all of them
+        int same = 0;
+        const int4* all = reinterpret_cast<const int4*>(e.index);
+#pragma unroll 4
+        for (int o = 0; o < entry_slots(g.topk) / 4; o++) {
+            const int4 x = all[o];
+            same += (x.x == i) + (x.y == i) + (x.z == i) + (x.w == i);
         }
-        if (first) dz[i] = grad_at(r, e.logit[j]) - w;
+        bool first = true;
+        float w = j == g.topk ? hard : soft == 0.f ? 0.f : soft * fast_exp2((e.value[j] - top) * kLog2e);
+        if (same > 1) {
+            w = 0.f;
+            for (int o = 0; o <= g.topk; o++) {
+                if (e.index[o] != i) continue;
+                if (o < j) { first = false; break; }
+                w += o == g.topk ? hard : soft == 0.f ? 0.f : soft * fast_exp2((e.value[o] - top) * kLog2e);
+            }
+        }
+        if (first) dz[i] = grad_at(r, g.w_hard != 0.f, e.logit[j]) - w;
     }
 }
 
-// ---- one workgroup per row: statistics, loss and (GRAD) gradient; NV * 4 floats a thread stay in registers between the two
-template <int THREADS, int NV, bool GRAD>
+// ---- one workgroup per row: statistics, loss and (GRAD) gradient.  Between the two a thread keeps NV vectors in registers and LV
+// in LDS; what is left of a long row streams through twice, the second time out of the memory-side cache.
+template <int THREADS, int NV, int LV, bool GRAD>
 __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillArgs g) {
-    extern __shared__ float lds[];
+    extern __shared__ __align__(16) float lds[];
     __shared__ float red[THREADS / 64][3];
     const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
     const Span part(g.z + row * g.ldz, 0, g.vocab);
     const bool hard = g.w_hard != 0.f;
+    f32x4* held = reinterpret_cast<f32x4*>(lds);
+    constexpr int GROUP = NV < 4 ? NV : 4, FIRST = (NV + LV) * THREADS;
+    // the row's entries are asked for before its logits: their own logits are then on the way behind those
+    const int slots = entry_slots(g.topk);
+    const Entries e = entries_at(lds + 4 * LV * THREADS, slots);
+    Entry mine(g, row, tid);
     f32x4 v[NV];
 #pragma unroll
-    for (int i = 0; i < NV; i++) v[i] = part.load(tid + i * THREADS);
+    for (int i = 0; i < NV; i++) v[i] = part.load<GRAD>(tid + i * THREADS);
     const float rest = part.rest(tid);
-    const Entries e = entries_at(lds, g.topk + 1);
-    stage_entries(g, row, e, part.z, nullptr, THREADS);
+    if (tid < slots) mine.stage(g, e, tid, g.z + row * g.ldz, 0, g.vocab);
+    for (int j = tid + THREADS; j < slots; j += THREADS) Entry(g, row, j).stage(g, e, j, g.z + row * g.ldz, 0, g.vocab);
     RowStats s = {-INFINITY, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < NV; i += 4) {
-        f32x4 u[4 < NV ? 4 : NV];
+    for (int i = 0; i < NV; i += GROUP) {
+        f32x4 u[GROUP];
 #pragma unroll
-        for (int q = 0; q < (4 < NV ? 4 : NV); q++) u[q] = v[i + q];
-        stats_of(u, g.cold, hard, s);
+        for (int q = 0; q < GROUP; q++) u[q] = v[i + q];
+        stats_of(u, g.cold, hard, g.power, s);
         __builtin_amdgcn_sched_barrier(0);
     }
-    for (int at = NV * THREADS + tid; at < part.vecs; at += 4 * THREADS) {
+    if constexpr (LV > 0) {
+#pragma unroll
+        for (int i = 0; i < LV; i += 3) {
+            f32x4 u[3];
+#pragma unroll
+            for (int q = 0; q < 3; q++) u[q] = part.load<GRAD>(tid + (NV + i + q) * THREADS);
+            stats_of(u, g.cold, hard, g.power, s);
+#pragma unroll
+            for (int q = 0; q < 3; q++) held[(i + q) * THREADS + tid] = u[q];
+        }
+    }
+    for (int at = FIRST + tid; at < part.vecs; at += 4 * THREADS) {
         f32x4 u[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) u[i] = part.load(at + i * THREADS);
-        stats_of(u, g.cold, hard, s);
+        stats_of(u, g.cold, hard, g.power, s);
     }
-    if (tid < part.tail) stats_of_one(rest, g.cold, s);
+    if (part.single(tid)) stats_of_one(rest, g.cold, s);
     s = block_stats<THREADS / 64>(s, g.cold, red);       // its barrier also publishes the entries
     float top, sum;
     teacher_softmax(g, e, top, sum);
-    if (tid < 64) {
-        const float l = row_loss_of(g, e, s, top, sum);
-        if (tid == 0) {
-            g.row_loss[row] = l;
-            if (g.stats) { g.stats[3 * row] = s.m; g.stats[3 * row + 1] = s.st; g.stats[3 * row + 2] = s.s1; }
-        }
-    }
+    if (tid < 64) finish_row(g, e, s, top, sum, row);
     if (!GRAD) return;
-    float* dz = g.dz + row * g.ldd;
+    float* dz = g.dz + row * g.ldd + part.head;
     const GradRow r = grad_row(g, e, s, sum);
     int again = tid;                                     // the stores' offsets are computed anew, not kept since the loads
     asm volatile("" : "+v"(again));
+    with_power(hard, g.power, [&](auto p) {
+        constexpr int POWER = decltype(p)::value;
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        grad_store(r, v[i], dz, again + i * THREADS, part.vecs);
-        __builtin_amdgcn_sched_barrier(0);               // four gradients in registers at a time, not all
-    }
-    for (int at = NV * THREADS + tid; at < part.vecs; at += 4 * THREADS) {
-        f32x4 u[4];
+        for (int i = 0; i < NV; i++) {
+            grad_store<POWER>(r, v[i], dz, again + i * THREADS, part.vecs);
+            __builtin_amdgcn_sched_barrier(0);           // four gradients in registers at a time, not all
+        }
+        if constexpr (LV > 0) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) u[i] = part.load(at + i * THREADS);
+            for (int i = 0; i < LV; i++) {
+                grad_store<POWER>(r, held[i * THREADS + tid], dz, again + (NV + i) * THREADS, part.vecs);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        for (int at = FIRST + tid; at < part.vecs; at += 4 * THREADS) {
+            f32x4 u[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) grad_store(r, u[i], dz, at + i * THREADS, part.vecs);
-    }
-    if (tid < part.tail) dz[4 * part.vecs + tid] = grad_at(r, rest);
+            for (int i = 0; i < 4; i++) u[i] = part.load(at + i * THREADS);
+#pragma unroll
+            for (int i = 0; i < 4; i++) grad_store<POWER>(r, u[i], dz, at + i * THREADS, part.vecs);
+        }
+    });
+    if (part.single(tid)) dz[part.place(tid)] = grad_at(r, hard, rest);
     __syncthreads();
-    grad_entries(g, e, r, top, sum, dz, 0, g.vocab, THREADS);
+    grad_entries(g, e, r, top, sum, g.dz + row * g.ldd, 0, g.vocab, THREADS);
 }
 
 // ---- rows cut into segments
@@ -291,9 +399,9 @@ __global__ __launch_bounds__(kSegThreads) void distill_segment_stats_kernel(Dist
         f32x4 u[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) u[i] = part.load(at + i * kSegThreads);
-        stats_of(u, g.cold, g.w_hard != 0.f, s);
+        stats_of(u, g.cold, g.w_hard != 0.f, g.power, s);
     }
-    if ((int)threadIdx.x < part.tail) stats_of_one(part.rest(threadIdx.x), g.cold, s);
+    if (part.single(threadIdx.x)) stats_of_one(part.rest(threadIdx.x), g.cold, s);
     s = block_stats<kSegThreads / 64>(s, g.cold, red);
     if (threadIdx.x == 0) {
         float* o = g.seg_stats + 3 * (row * g.segments + blockIdx.x);
@@ -323,18 +431,12 @@ __global__ __launch_bounds__(kSegThreads) void distill_segment_grad_kernel(Disti
     const int64_t row = blockIdx.y;
     const int begin = GRAD ? blockIdx.x * g.per_segment : 0, end = GRAD ? min(g.vocab, begin + g.per_segment) : 0;
     const float* z = g.z + row * g.ldz;
-    const Entries e = entries_at(lds, g.topk + 1);
-    if (JOIN) {
-        stage_entries(g, row, e, z, g.seg_logit, kSegThreads);
-    } else {
-        // only this segment's logits: others' may be overwritten already
-        for (int j = threadIdx.x; j <= g.topk; j += kSegThreads) {
-            int i = j < g.topk ? g.index[row * g.topk + j] : g.labels ? g.labels[row] : -1;
-            if (i < 0 || i >= g.vocab) i = -1;
-            e.index[j] = i;
-            e.value[j] = j < g.topk && i >= 0 ? g.teacher[row * g.topk + j] * g.inv_t : -INFINITY;
-            e.logit[j] = i >= begin && i < end ? z[i] : 0.f;
-        }
+    const int slots = entry_slots(g.topk);
+    const Entries e = entries_at(lds, slots);
+    for (int j = threadIdx.x; j < slots; j += kSegThreads) {
+        Entry x(g, row, j);
+        x.stage(g, e, j, z, begin, JOIN ? 0 : end);      // only this segment's logits: others' may be overwritten already
+        if (JOIN && j <= g.topk && x.index >= 0) e.logit[j] = g.seg_logit[row * (g.topk + 1) + j];
     }
     RowStats s;
     if (JOIN) s = joined_stats(g, row);
@@ -342,42 +444,23 @@ __global__ __launch_bounds__(kSegThreads) void distill_segment_grad_kernel(Disti
     __syncthreads();
     float top, sum;
     teacher_softmax(g, e, top, sum);
-    if (JOIN && blockIdx.x == 0 && threadIdx.x < 64) {
-        const float l = row_loss_of(g, e, s, top, sum);
-        if (threadIdx.x == 0) {
-            g.row_loss[row] = l;
-            if (g.stats) { g.stats[3 * row] = s.m; g.stats[3 * row + 1] = s.st; g.stats[3 * row + 2] = s.s1; }
-        }
-    }
+    if (JOIN && blockIdx.x == 0 && threadIdx.x < 64) finish_row(g, e, s, top, sum, row);
     if (!GRAD) return;
     float* dz = g.dz + row * g.ldd;
     const GradRow r = grad_row(g, e, s, sum);
     const Span part(z, begin, end);
-    for (int at = threadIdx.x; at < part.vecs; at += 4 * kSegThreads) {
-        f32x4 u[4];
+    with_power(g.w_hard != 0.f, g.power, [&](auto p) {
+        for (int at = threadIdx.x; at < part.vecs; at += 4 * kSegThreads) {
+            f32x4 u[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) u[i] = part.load(at + i * kSegThreads);
+            for (int i = 0; i < 4; i++) u[i] = part.load(at + i * kSegThreads);
 #pragma unroll
-        for (int i = 0; i < 4; i++) grad_store(r, u[i], dz + begin, at + i * kSegThreads, part.vecs);
-    }
-    if ((int)threadIdx.x < part.tail) dz[begin + 4 * part.vecs + threadIdx.x] = grad_at(r, part.rest(threadIdx.x));
+            for (int i = 0; i < 4; i++) grad_store<decltype(p)::value>(r, u[i], dz + begin + part.head, at + i * kSegThreads, part.vecs);
+        }
+    });
+    if (part.single(threadIdx.x)) dz[begin + part.head + part.place(threadIdx.x)] = grad_at(r, g.w_hard != 0.f, part.rest(threadIdx.x));
     __syncthreads();
     grad_entries(g, e, r, top, sum, dz, begin, end, kSegThreads);
-}
-
-// loss = scale * sum of the rows' losses, in a fixed order
-__global__ __launch_bounds__(1024) void distill_loss_kernel(const float* __restrict__ row_loss, int64_t rows, float scale, float* out) {
-    __shared__ double red[16];
-    double s = 0.0;
-    for (int64_t i = threadIdx.x; i < rows; i += 1024) s += (double)row_loss[i];
-    s = wave_sum_f64(s);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double t = 0.0;
-        for (int i = 0; i < 16; i++) t += red[i];
-        out[0] = (float)(t * (double)scale);
-    }
 }
 
 static int distill_check(const char* fn, const float* z, int64_t ldz, const float* teacher, const int32_t* index, int64_t rows, int64_t vocab,
@@ -399,6 +482,7 @@ static DistillArgs distill_args(const float* z, int64_t ldz, const float* teache
     g.rows = rows; g.vocab = (int)vocab; g.topk = (int)topk;
     g.inv_t = 1.f / temperature;
     g.cold = kLog2e / temperature;
+    g.power = temperature == 1.f ? 1 : temperature == 2.f ? 2 : temperature == 3.f ? 3 : temperature == 4.f ? 4 : 0;
     g.w_soft = alpha * temperature * temperature;
     g.w_hard = labels ? 1.f - alpha : 0.f;
     g.g_soft = scale * alpha * temperature;
@@ -417,19 +501,35 @@ static void cut_row(DistillArgs& g, int segments) {
     g.segments = (int)ceil_div(g.vocab, g.per_segment);
 }
 
+template <int THREADS, int NV, int LV, bool GRAD>
+static int launch_row_kernel(const DistillArgs& g) {
+    const size_t bytes = sizeof(float) * (4 * (size_t)LV * THREADS + 3 * (size_t)entry_slots(g.topk));
+    static size_t raised = 64 * 1024;
+    if (bytes > raised) {
+        const int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(&distill_row_kernel<THREADS, NV, LV, GRAD>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "bh_distill: LDS size");
+        if (rc) return rc;
+        raised = bytes;
+    }
+    hipLaunchKernelGGL((distill_row_kernel<THREADS, NV, LV, GRAD>), dim3((unsigned)g.rows), dim3(THREADS), bytes, stream(), g);
+    return BH_LAUNCH_CHECK("bh_distill");
+}
+
+// Threads and registers per row, by the row's length: a row that fits wholly is read once; with 512 threads and LDS two rows of
+// 51 K logits share a compute unit, one being read while the other is worked on.  Loss and gradient on 4096 to 16384 rows, us:
+//   758 logits   17 with 64 x 4 vectors, 20 with 128 x 4, 26 with 256 x 4      2000   54 with 128 x 4, 59 with 256 x 4
+//   8000   213 with 256 x 8, 236 with 512 x 8      16000   200 with 512 x 8, 221 with 256 x 8, 246 with LDS
+//   32000  194 with LDS, 205 with 512 x 8          50001   683 with LDS, 761 with 512 x 8, 810 with 1024 x 8
+// The loss alone reads the row once anyway.
 template <bool GRAD>
 static int launch_rows(const DistillArgs& g) {
-    const size_t lds = sizeof(float) * 3 * (size_t)(g.topk + 1);
-    const dim3 grid((unsigned)g.rows);
-    // the gradient's rows stay in registers (as many threads as it takes, up to the 64 K floats of a compute unit); without
-    // one the row only streams through
-    if (!GRAD && g.vocab > 4096) hipLaunchKernelGGL((distill_row_kernel<512, 8, GRAD>), grid, dim3(512), lds, stream(), g);
-    else if (g.vocab <= 1024) hipLaunchKernelGGL((distill_row_kernel<256, 1, GRAD>), grid, dim3(256), lds, stream(), g);
-    else if (g.vocab <= 4096) hipLaunchKernelGGL((distill_row_kernel<256, 4, GRAD>), grid, dim3(256), lds, stream(), g);
-    else if (g.vocab <= 16384) hipLaunchKernelGGL((distill_row_kernel<256, 16, GRAD>), grid, dim3(256), lds, stream(), g);
-    else if (g.vocab <= 32768) hipLaunchKernelGGL((distill_row_kernel<512, 16, GRAD>), grid, dim3(512), lds, stream(), g);
-    else hipLaunchKernelGGL((distill_row_kernel<1024, 16, GRAD>), grid, dim3(1024), lds, stream(), g);
-    return BH_LAUNCH_CHECK("bh_distill");
+    if (g.vocab <= 1024) return launch_row_kernel<64, 4, 0, GRAD>(g);
+    if (g.vocab <= 2048) return launch_row_kernel<128, 4, 0, GRAD>(g);
+    if (g.vocab <= 4096) return launch_row_kernel<256, 4, 0, GRAD>(g);
+    if (!GRAD) return launch_row_kernel<512, 8, 0, GRAD>(g);
+    if (g.vocab <= 8192) return launch_row_kernel<256, 8, 0, true>(g);
+    if (g.vocab <= 24576) return launch_row_kernel<512, 8, 0, true>(g);
+    return launch_row_kernel<512, 16, 9, true>(g);
 }
 
 template <bool GRAD>
@@ -452,7 +552,7 @@ static int run_distill(DistillArgs g, float scale, float* loss_out) {
         hipLaunchKernelGGL(distill_segment_stats_kernel, dim3((unsigned)g.segments, (unsigned)g.rows), dim3(kSegThreads), 0, stream(), g);
         rc = BH_LAUNCH_CHECK("bh_distill: segments");
         if (rc) return rc;
-        const size_t lds = sizeof(float) * 3 * (size_t)(g.topk + 1);
+        const size_t lds = sizeof(float) * 3 * (size_t)entry_slots(g.topk);
         hipLaunchKernelGGL((distill_segment_grad_kernel<true, GRAD>), dim3(GRAD ? (unsigned)g.segments : 1u, (unsigned)g.rows),
                            dim3(kSegThreads), lds, stream(), g);
         rc = BH_LAUNCH_CHECK("bh_distill: join");
@@ -496,7 +596,7 @@ int bh_distill_backward(const float* logits, int64_t ld, const float* teacher, c
     // a workgroup streams a segment of at most 16 K logits; the grid's second dimension holds 65535 rows
     const int64_t by_size = ceil_div(vocab, 16384), by_rows = segments_for(rows, vocab);
     cut_row(g, (int)(by_size > by_rows ? by_size : by_rows));
-    const size_t lds = sizeof(float) * 3 * (size_t)(topk + 1);
+    const size_t lds = sizeof(float) * 3 * (size_t)entry_slots((int)topk);
     for (int64_t r0 = 0; r0 < rows; r0 += 65535) {
         DistillArgs h = g;
         h.rows = rows - r0 < 65535 ? rows - r0 : 65535;
