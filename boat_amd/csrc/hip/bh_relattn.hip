@@ -32,6 +32,7 @@ constexpr float kMaskedBias = -1e30f;      // a table value this low masks its b
 struct Buckets {
     int exact, far, side, last;            // far: logarithmic buckets; side: buckets of one direction; last = border[far - 1]
     int both;
+    int line;                              // relative positions from the last border (and a block) on one side to the other's, or 0
     float log2_exact, per_log2;
     int border[kMaxBuckets / 2 + 1];
 };
@@ -57,44 +58,74 @@ struct RelArgs {
     Buckets b;
 };
 
-// ---- the bias as a wavefront sees it; border and value live in LDS
-struct Bias {
-    const int* border;
-    const float* value;                    // the head's table column times log2 e
-    __device__ __forceinline__ int bucket(const Buckets& b, int rel) const {
-        const int n = b.both ? abs(rel) : max(-rel, 0);
-        int f = (int)((__builtin_amdgcn_logf((float)max(n, 1)) - b.log2_exact) * b.per_log2);   // right up to one, the borders decide
-        f = min(max(f, 0), b.far - 1);
-        if (n < border[f]) f--;
-        else if (n >= border[f + 1]) f++;  // border[far] is past every distance
-        const int one = n < b.exact ? n : b.exact + f;
-        return b.both && rel > 0 ? b.side + one : one;
-    }
-};
+// ---- the bias as a workgroup sees it.  Where the borders span no more than kLine relative positions LDS holds the bias (times
+// log2 e) and the bucket of each of them, worked out once; else the borders and the head's table column, and every wavefront
+// looks its blocks' diagonals up.
+constexpr int kLine = 1024;
+
+__device__ __forceinline__ int bucket_of(const Buckets& b, const int* border, int rel) {
+    const int n = b.both ? abs(rel) : max(-rel, 0);
+    int f = (int)((__builtin_amdgcn_logf((float)max(n, 1)) - b.log2_exact) * b.per_log2);   // right up to one, the borders decide
+    f = min(max(f, 0), b.far - 1);
+    if (n < border[f]) f--;
+    else if (n >= border[f + 1]) f++;      // border[far] is past every distance
+    const int one = n < b.exact ? n : b.exact + f;
+    return b.both && rel > 0 ? b.side + one : one;
+}
+__device__ __forceinline__ float table_value(const RelArgs& g, int bucket, int head) {
+    const float t = g.table[(int64_t)bucket * g.heads + head];
+    return t <= kMaskedBias ? -INFINITY : t * kLog2e;
+}
 // does every relative position of [lo, hi] fall into one bucket?  Which one, or -1
 __device__ __forceinline__ int constant_bucket(const Buckets& b, int64_t lo, int64_t hi) {
     if (hi <= -(int64_t)b.last) return b.side - 1;
     if (b.both) return lo >= b.last ? 2 * b.side - 1 : -1;
     return lo >= 0 ? 0 : -1;
 }
-__device__ __forceinline__ float table_value(const RelArgs& g, int bucket, int head) {
-    const float t = g.table[(int64_t)bucket * g.heads + head];
-    return t <= kMaskedBias ? -INFINITY : t * kLog2e;
-}
-__device__ __forceinline__ void stage_bias(const RelArgs& g, int head, int* border, float* value, int threads) {
-    for (int i = threadIdx.x; i <= g.b.far; i += threads) border[i] = g.b.border[i];
-    for (int i = threadIdx.x; i < g.buckets; i += threads) value[i] = table_value(g, i, head);
-}
-// relative positions base - 31 .. base + 31 of a block (and one more): a lane's bucket, the values in win[64]
-__device__ __forceinline__ int stage_window(const Buckets& b, const Bias& bias, int64_t base, float* win, int lane) {
-    const int k = bias.bucket(b, (int)(base + lane - 31));
-    __builtin_amdgcn_wave_barrier();
-    win[lane] = bias.value[k];
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    return k;
-}
+struct Bias {
+    static constexpr int WINDOW = 4 * (kMaxBuckets / 2 + 4) + 4 * kMaxBuckets;   // borders and column, then 64 floats a wavefront
+    static constexpr int BYTES = 5 * kLine;
+    static_assert(WINDOW + 4 * 64 * 4 <= BYTES, "four wavefronts");
+
+    char* lds;
+    int first;                             // relative position of the line's start
+    float before, behind;                  // past the last border: keys before the query, keys behind it
+    bool line;
+
+    // to be followed by a barrier
+    __device__ __forceinline__ Bias(const RelArgs& g, int head, char* area, int threads)
+        : lds(area), first(-(g.b.last + 63)), before(table_value(g, g.b.side - 1, head)),
+          behind(table_value(g, g.b.both ? 2 * g.b.side - 1 : 0, head)), line(g.b.line > 0) {
+        if (line) {
+            for (int i = threadIdx.x; i < g.b.line; i += threads) {
+                const int k = bucket_of(g.b, g.b.border, first + i);
+                reinterpret_cast<float*>(lds)[i] = table_value(g, k, head);
+                reinterpret_cast<unsigned char*>(lds)[4 * kLine + i] = (unsigned char)k;
+            }
+        } else {
+            int* border = reinterpret_cast<int*>(lds);
+            float* value = reinterpret_cast<float*>(lds + 4 * (kMaxBuckets / 2 + 4));
+            for (int i = threadIdx.x; i <= g.b.far; i += threads) border[i] = g.b.border[i];
+            for (int i = threadIdx.x; i < g.buckets; i += threads) value[i] = table_value(g, i, head);
+        }
+    }
+    __device__ __forceinline__ int bucket(const Buckets& b, int rel) const {
+        return line ? reinterpret_cast<const unsigned char*>(lds)[4 * kLine + rel - first] : bucket_of(b, reinterpret_cast<const int*>(lds), rel);
+    }
+    // the biases of relative positions rel0 - 31 .. rel0 + 31 (a block that is not constant), for one wavefront
+    __device__ __forceinline__ const float* diagonals(const Buckets& b, int rel0, int wave, int lane) const {
+        if (line) return reinterpret_cast<const float*>(lds) + (rel0 - 31 - first);
+        const float* value = reinterpret_cast<const float*>(lds + 4 * (kMaxBuckets / 2 + 4));
+        float* win = reinterpret_cast<float*>(lds + WINDOW) + 64 * wave;
+        const float t = value[bucket_of(b, reinterpret_cast<const int*>(lds), rel0 + lane - 31)];
+        __builtin_amdgcn_wave_barrier();
+        win[lane] = t;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        return win;
+    }
+};
 
 // ---- loading.  Eight floats of a row from element c on; places past d, and rows that are not `live`, are zero
 __device__ __forceinline__ void row_eight(const float* __restrict__ p, bool live, int c, int d, bool vec, float (&x)[8]) {
@@ -133,6 +164,7 @@ struct SplitJob {
     int blocks;                                          // of 32 rows, per head
     char* row; char* col;                                // either may be NULL
     bool vec;
+    const float* with; float* dots;                      // dots [head][row] = the row's product with the same row of `with`, or NULL
 };
 constexpr int kMaxJobs = 4;
 struct SplitJobs { SplitJob j[kMaxJobs]; int first[kMaxJobs + 1]; int d; };   // first: workgroup number at which a job starts
@@ -165,6 +197,17 @@ __global__ __launch_bounds__(256) void relattn_split_kernel(SplitJobs a) {
         *reinterpret_cast<f32x4*>(&x[r][c]) = v;
     }
     __syncthreads();
+    if (j.dots) {                                        // eight lanes a row
+        const int r = threadIdx.x >> 3;
+        float t = 0.f;
+        if (r < live) {
+            const float* w = j.with + bt * j.s[0] + h * j.s[1] + (row0 + r) * j.s[2];
+            for (int c = threadIdx.x & 7; c < a.d; c += 8) t += x[r][c] * w[c];
+        }
+#pragma unroll
+        for (int off = 4; off > 0; off >>= 1) t += __shfl_xor(t, off, 64);
+        if (r < live && (threadIdx.x & 7) == 0) j.dots[(int64_t)bh * j.rows + row0 + r] = t;
+    }
     const int64_t at = ((int64_t)bh * j.blocks + blk) * Block<DP>::BYTES;
     if (j.row)
         for (int i = threadIdx.x; i < 32 * (DP / 8); i += 256) {
@@ -241,29 +284,28 @@ __device__ __forceinline__ f32x16 zero16() {
 }
 
 // scores of a block [32 keys as rows][32 queries as columns] in log2 units: scaled, biased, masked.  rel0 = first key - first
-// query position; key_last = last valid key's row in the block; q = this lane's query's column
-__device__ __forceinline__ void finish_scores(const RelArgs& g, const Bias& bias, f32x16& s, float c, int64_t rel0, int64_t keys_left, float* win,
-                                              int lane, int& bucket, int& constant) {
-    constant = constant_bucket(g.b, rel0 - 31, rel0 + 31);
+// query position; keys_left = valid keys from the block's first on.  Returns the bucket all of it falls into, or -1
+__device__ __forceinline__ int finish_scores(const RelArgs& g, const Bias& bias, f32x16& s, float c, int rel0, int keys_left, int wave, int lane) {
+    const int constant = constant_bucket(g.b, rel0 - 31, rel0 + 31);
     if (constant >= 0) {
-        const float t = bias.value[constant];
+        const float t = constant == g.b.side - 1 ? bias.before : bias.behind;
 #pragma unroll
         for (int e = 0; e < 16; e++) s[e] = fmaf(s[e], c, t);
     } else {
-        bucket = stage_window(g.b, bias, rel0, win, lane);
-        const float* w = win + 31 - (lane & 31) + 4 * (lane >> 5);
+        const float* w = bias.diagonals(g.b, rel0, wave, lane) + 31 - (lane & 31) + 4 * (lane >> 5);
 #pragma unroll
         for (int e = 0; e < 16; e++) s[e] = fmaf(s[e], c, w[8 * (e >> 2) + (e & 3)]);
     }
     if (keys_left < 32 || (g.causal && rel0 + 31 > 0)) {
         // a key is seen when its row is below keys_left and, causal, rel0 + row - column <= 0
-        int64_t lim = min(keys_left, (int64_t)32);
+        int lim = min(keys_left, 32);
         if (g.causal) lim = min(lim, (lane & 31) - rel0 + 1);
-        const int own = (int)max(lim, (int64_t)0) - 4 * (lane >> 5);
+        const int own = lim - 4 * (lane >> 5);
 #pragma unroll
         for (int e = 0; e < 16; e++)
             if (8 * (e >> 2) + (e & 3) >= own) s[e] = -INFINITY;
     }
+    return constant;
 }
 
 // workgroup number -> (batch*head, tile): the tiles of one head stay on one XCD, whose L2 then holds its keys and values;
@@ -347,10 +389,8 @@ __device__ __forceinline__ void running_softmax(f32x16 (&s)[NB], float& m, float
 template <int DP> struct ForwardLds {
     static constexpr int NB = DP <= 64 ? 2 : 1;                               // blocks of 32 keys a step
     static constexpr int V = NB * Block<DP>::BYTES;
-    static constexpr int BORDER = 2 * V;
-    static constexpr int VALUE = BORDER + 4 * (kMaxBuckets / 2 + 4);
-    static constexpr int WIN = VALUE + 4 * kMaxBuckets;
-    static constexpr int BYTES = WIN + kWaves * 64 * 4;
+    static constexpr int BIAS = 2 * V;
+    static constexpr int BYTES = BIAS + Bias::BYTES;
 };
 
 // A workgroup owns 128 queries of a head, a wavefront 32 of them, and walks over the keys.  Keys and values have a place in
@@ -360,18 +400,14 @@ __global__ __launch_bounds__(kThreads, 2) void relattn_forward_kernel(RelArgs g)
     using L = ForwardLds<DP>;
     constexpr int NB = L::NB, KEYS = 32 * NB, ND = DP / 32, KD = DP / 16;
     extern __shared__ __align__(16) char smem[];
-    int* border = reinterpret_cast<int*>(smem + L::BORDER);
-    float* value = reinterpret_cast<float*>(smem + L::VALUE);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    float* win = reinterpret_cast<float*>(smem + L::WIN) + 64 * wave;
     int bh, tile;
     head_and_tile(blockIdx.x, g.batch * g.heads, g.q_tiles, bh, tile);
     const int bt = bh / g.heads, h = bh % g.heads, hk = h / g.group;
     const float* q = g.q + bt * g.qs[0] + h * g.qs[1];
     const int64_t plane0 = ((int64_t)bt * g.kv_heads + hk) * g.k_blocks * Block<DP>::BYTES;
     const char *kp = g.k_row + plane0, *vp = g.v_col + plane0;
-    stage_bias(g, h, border, value, kThreads);
-    const Bias bias = {border, value};
+    const Bias bias(g, h, smem + L::BIAS, kThreads);
 
     const int q0 = tile * kQueryTile, qw = q0 + 32 * wave;                    // this wavefront's queries: qw + 0..31
     const int qi = qw + (lane & 31);
@@ -411,10 +447,7 @@ __global__ __launch_bounds__(kThreads, 2) void relattn_forward_kernel(RelArgs g)
             copy_to_lds<2 * NB * DP * 96 / 1024, kWaves>(kp + (int64_t)((k0 + KEYS) / 32) * Block<DP>::BYTES, smem, wave, lane);
         if (mine) {
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                int bucket, constant;
-                finish_scores(g, bias, s[b], c, k0 + 32 * b - rel_q, ke - k0 - 32 * b, win, lane, bucket, constant);
-            }
+            for (int b = 0; b < NB; b++) finish_scores(g, bias, s[b], c, k0 + 32 * b - rel_q, ke - k0 - 32 * b, wave, lane);
             running_softmax(s, m, l, o);
             u32x4 p[kPlanes];
             pipelined<2 * NB * ND>([&](int i, u32x4 (&a)[kPlanes]) {
@@ -449,7 +482,6 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 96 ? 2 : 1) void relattn_rows
     const float* v = g.v + bt * g.vs[0] + hk * g.vs[1];
     for (int i = tid; i <= g.b.far; i += 64 * kRowWaves) border[i] = g.b.border[i];
     __syncthreads();
-    const Bias bias = {border, nullptr};
     const int len = g.kv_len ? min(max(g.kv_len[bt], 0), (int)g.sk) : (int)g.sk;
     const int kb = (int)min((int64_t)len, blockIdx.y * g.keys_per_split), ke = (int)min((int64_t)len, kb + g.keys_per_split);
     const int pos = (int)(qi + g.offset);
@@ -495,7 +527,7 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 96 ? 2 : 1) void relattn_rows
             for (int e = 0; e < 16; e++) s[0][e] = fmaf(s[0][e], c, t);
         } else {
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[0][e] = fmaf(s[0][e], c, table_value(g, bias.bucket(g.b, rel0 + acc_row(e, lane)), h));
+            for (int e = 0; e < 16; e++) s[0][e] = fmaf(s[0][e], c, table_value(g, bucket_of(g.b, border, rel0 + acc_row(e, lane)), h));
         }
         int lim = ke - k0;
         if (g.causal) lim = min(lim, 1 - rel0);
@@ -547,56 +579,45 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 96 ? 2 : 1) void relattn_rows
     if (wave == 0 && 32 * rt + (lane & 31) < rows) store_forward<DP>(g, o, top, sum, bt * g.heads + h, qi, blockIdx.y, lane);
 }
 
-// the splits' parts of a row: one wavefront per row
+// the splits' parts of a row: one wavefront per row, a lane per split (at most 64) for the weights
 __global__ __launch_bounds__(256) void relattn_join_kernel(RelArgs g) {
     const int64_t rows = (int64_t)g.batch * g.heads * g.sq;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= rows) return;
-    float m = -INFINITY;
-    for (int s = lane; s < g.splits; s += 64) m = fmaxf(m, g.part_ml[2 * (s * rows + row)]);
-    m = wave_max(m);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int s = lane; s < g.splits; s += 64) l += g.part_ml[2 * (s * rows + row) + 1] * __builtin_amdgcn_exp2f(g.part_ml[2 * (s * rows + row)] - base);
-    l = wave_sum(l);
+    float m = -INFINITY, l = 0.f;
+    if (lane < g.splits) {
+        const f32x2 ml = *reinterpret_cast<const f32x2*>(g.part_ml + 2 * (lane * rows + row));
+        m = ml[0];
+        l = ml[1];
+    }
+    const float top = wave_max(m), base = top == -INFINITY ? 0.f : top;
+    const float w = __builtin_amdgcn_exp2f(m - base);                         // 0 for a lane without a split
+    const float sum = wave_sum(l * w);
     const int64_t bh = row / g.sq, qi = row % g.sq;
     float* dst = g.out + bh / g.heads * g.os[0] + bh % g.heads * g.os[1] + qi * g.os[2];
-    const float f = m == -INFINITY ? 0.f : 1.f / l;
-    for (int c = lane; c < g.d; c += 64) {
+    const float f = top == -INFINITY ? 0.f : 1.f / sum;
+    for (int c = lane; c < (g.d + 63) / 64 * 64; c += 64) {
+        const float* p = g.part_o + row * g.d + min(c, g.d - 1);
         float a = 0.f;
+#pragma unroll 8
         for (int s = 0; s < g.splits; s++) {
-            const float w = __builtin_amdgcn_exp2f(g.part_ml[2 * (s * rows + row)] - base);
-            a += w == 0.f ? 0.f : w * g.part_o[(s * rows + row) * g.d + c];
+            const float x = p[s * rows * g.d], y = __shfl(w, s, 64);
+            a += y == 0.f ? 0.f : y * x;
         }
-        dst[c] = a * f;
+        if (c < g.d) dst[c] = a * f;
     }
-    if (lane == 0) g.lse[row] = m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    if (lane == 0) g.lse[row] = top == -INFINITY ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------------------------------- backward
-// delta = rowsum(dO o O): one wavefront per four rows, 16 lanes a row
-__global__ __launch_bounds__(256) void relattn_delta_kernel(RelArgs g) {
-    const int64_t rows = (int64_t)g.batch * g.heads * g.sq;
-    const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (row >= rows) return;
-    const int64_t bh = row / g.sq, qi = row % g.sq, at = bh / g.heads * g.os[0] + bh % g.heads * g.os[1] + qi * g.os[2];
-    float s = 0.f;
-    for (int c = threadIdx.x & 15; c < g.d; c += 16) s += g.out_in[at + c] * g.d_out[at + c];
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-    if ((threadIdx.x & 15) == 0) g.delta[row] = s;
-}
-
 // log2 e * lse; rows that see nothing get a number (their scores are all masked)
 __device__ __forceinline__ float lse_log2(float lse) { return lse == -INFINITY ? 0.f : lse * kLog2e; }
 
 template <int DP> struct QueryLds {
     static constexpr int V = Block<DP>::BYTES, KT = 2 * Block<DP>::BYTES;     // keys and values in row form, keys in column form
-    static constexpr int BORDER = 3 * Block<DP>::BYTES;
-    static constexpr int VALUE = BORDER + 4 * (kMaxBuckets / 2 + 4);
-    static constexpr int WIN = VALUE + 4 * kMaxBuckets;
-    static constexpr int SUMS = WIN + kWaves * 64 * 4;                        // per wavefront: a sum per bucket, in 64 bits
+    static constexpr int BIAS = 3 * Block<DP>::BYTES;
+    static constexpr int SUMS = BIAS + Bias::BYTES;                           // per wavefront: a sum per bucket, in 64 bits
     static constexpr int BLOCK = SUMS + kWaves * kMaxBuckets * 8;             // per wavefront: a block of dS, rows of 33
     static constexpr int BYTES = BLOCK + kWaves * 32 * 33 * 4;
 };
@@ -607,10 +628,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
     using L = QueryLds<DP>;
     constexpr int KEYS = 32, ND = DP / 32, KD = DP / 16, KB = Block<DP>::BYTES / 1024;
     extern __shared__ __align__(16) char smem[];
-    int* border = reinterpret_cast<int*>(smem + L::BORDER);
-    float* value = reinterpret_cast<float*>(smem + L::VALUE);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    float* win = reinterpret_cast<float*>(smem + L::WIN) + 64 * wave;
     double* sums = reinterpret_cast<double*>(smem + L::SUMS) + kMaxBuckets * wave;
     float* block = reinterpret_cast<float*>(smem + L::BLOCK) + 32 * 33 * wave;
     int bh, tile;
@@ -619,9 +637,8 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
     const float* q = g.q + bt * g.qs[0] + h * g.qs[1];
     const float* dout = g.d_out + bt * g.os[0] + h * g.os[1];
     const int64_t plane0 = ((int64_t)bt * g.kv_heads + hk) * g.k_blocks * Block<DP>::BYTES;
-    stage_bias(g, h, border, value, kThreads);
+    const Bias bias(g, h, smem + L::BIAS, kThreads);
     for (int i = lane; i < g.buckets; i += 64) sums[i] = 0.0;
-    const Bias bias = {border, value};
 
     const int q0 = tile * kQueryTile, qw = q0 + 32 * wave, qi = qw + (lane & 31);
     const bool live = qi < g.sq;
@@ -678,8 +695,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
         wait_copies();
         if (k0 + KEYS < ke) fetch_rows(k0 + KEYS);
         if (mine) {
-        int bucket = 0, constant;
-        finish_scores(g, bias, s, c, k0 - rel_q, ke - k0, win, lane, bucket, constant);
+        const int constant = finish_scores(g, bias, s, c, k0 - rel_q, ke - k0, wave, lane);
 #pragma unroll
         for (int e = 0; e < 16; e++) s[e] = live ? __builtin_amdgcn_exp2f(s[e] - lse) * fmaf(dp[e], sign, -delta) : 0.f;
         if (constant >= 0) {
@@ -690,6 +706,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
             if (constant == g.b.side - 1) far_sum[0] += all; else far_sum[1] += all;
         } else {
             // diagonal `lane` of the block: key row r, query column x with r - x = lane - 31
+            const int bucket = bias.bucket(g.b, k0 - rel_q + lane - 31);
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int e = 0; e < 16; e++) block[acc_row(e, lane) * 33 + (lane & 31)] = s[e];
@@ -783,10 +800,8 @@ template <int DP> struct KeyLds {
     static constexpr int G = Block<DP>::BYTES;                                // queries and dO: row form, then column form
     static constexpr int QT = 2 * G, GT = 3 * G;
     static constexpr int STAT = 4 * G;                                        // lse and delta of a step's queries, twice
-    static constexpr int BORDER = STAT + 2 * 64 * 4;
-    static constexpr int VALUE = BORDER + 4 * (kMaxBuckets / 2 + 4);
-    static constexpr int WIN = VALUE + 4 * kMaxBuckets;
-    static constexpr int BYTES = WIN + kWaves * 64 * 4;
+    static constexpr int BIAS = STAT + 2 * 64 * 4;
+    static constexpr int BYTES = BIAS + Bias::BYTES;
 };
 
 // dK and dV of one query head: a workgroup owns 128 keys and walks over the queries.  Heads that share a key head leave their
@@ -796,10 +811,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
     using L = KeyLds<DP>;
     constexpr int ROWS = 32, ND = DP / 32, KD = DP / 16, KB = Block<DP>::BYTES / 1024;
     extern __shared__ __align__(16) char smem[];
-    int* border = reinterpret_cast<int*>(smem + L::BORDER);
-    float* value = reinterpret_cast<float*>(smem + L::VALUE);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    float* win = reinterpret_cast<float*>(smem + L::WIN) + 64 * wave;
     int bh, tile;
     head_and_tile(blockIdx.x, g.batch * g.heads, k_tiles, bh, tile);
     tile = k_tiles - 1 - tile;                                                // the first keys are seen by the most queries
@@ -842,14 +854,16 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
                 reinterpret_cast<float*>(smem + L::STAT)[64 * buffer + tid] = tid < ROWS ? lse_log2(g.lse_in[row0 + r]) : g.delta[row0 + r];
             }
         };
-        stage_bias(g, h, border, value, kThreads);
-        const Bias bias = {border, value};
-        fetch(g.q_row, g.g_row, qb, 0);
-        fetch_stat(qb, 0);
+        const Bias bias(g, h, smem + L::BIAS, kThreads);
+        // from the last queries down: under a causal mask, where the key tiles have different first queries, all the workgroups
+        // of a head are then at the same queries at the same time and read them out of the L2 once
+        const int q_last = (sq - 1) / ROWS * ROWS;
+        fetch(g.q_row, g.g_row, q_last, 0);
+        fetch_stat(q_last, 0);
         wait_copies();
-        for (int r0 = qb, turn = 0; r0 < sq; r0 += ROWS, turn ^= 1) {
+        for (int r0 = q_last, turn = 0; r0 >= qb; r0 -= ROWS, turn ^= 1) {
             fetch(g.q_col, g.g_col, r0, L::QT);
-            if (r0 + ROWS < sq) fetch_stat(r0 + ROWS, turn ^ 1);
+            if (r0 > qb) fetch_stat(r0 - ROWS, turn ^ 1);
             const float* stat = reinterpret_cast<const float*>(smem + L::STAT) + 64 * turn;
             const bool mine = kw < len && !(g.causal && kw > min(r0 + ROWS, sq) - 1 + g.offset);
             f32x16 s, dp;
@@ -863,19 +877,18 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
                                   });
             }
             wait_copies();
-            if (r0 + ROWS < sq) fetch(g.q_row, g.g_row, r0 + ROWS, 0);
+            if (r0 > qb) fetch(g.q_row, g.g_row, r0 - ROWS, 0);
             if (mine) {
             // block [32 queries as rows][32 keys as columns]
             const int rel0 = (int)(kw - r0 - g.offset);
             const int constant = constant_bucket(g.b, rel0 - 31, rel0 + 31);
             const f32x4* ls = reinterpret_cast<const f32x4*>(stat + 4 * (lane >> 5));   // lse of rows 8g + 4 half + 0..3
             if (constant >= 0) {
-                const float t = value[constant];
+                const float t = constant == g.b.side - 1 ? bias.before : bias.behind;
 #pragma unroll
                 for (int e = 0; e < 16; e++) s[e] = fmaf(s[e], c, t - ls[2 * (e >> 2)][e & 3]);
             } else {
-                stage_window(g.b, bias, rel0, win, lane);
-                const float* w = win + (lane & 31) - 4 * (lane >> 5) + 4;
+                const float* w = bias.diagonals(g.b, rel0, wave, lane) + (lane & 31) - 4 * (lane >> 5) + 4;
 #pragma unroll
                 for (int e = 0; e < 16; e++) s[e] = fmaf(s[e], c, w[27 - 8 * (e >> 2) - (e & 3)] - ls[2 * (e >> 2)][e & 3]);
             }
@@ -975,6 +988,8 @@ static bool make_buckets(int num, int distance, int both, Buckets& b) {
     }
     b.border[b.far] = 0x7fffffff;
     b.last = b.border[b.far - 1];
+    const int64_t line = (b.both ? 2 : 1) * (int64_t)b.last + 128;
+    b.line = line <= kLine ? (int)line : 0;
     return true;
 }
 
@@ -1051,6 +1066,7 @@ struct Planes {
         total += batch * heads * blocks;
         for (int i = ++n; i <= kMaxJobs; i++) jobs.first[i] = total;
     }
+    SplitJob& last() { return jobs.j[n - 1]; }
     template <int DP> int launch(int d) {
         jobs.d = d;
         hipLaunchKernelGGL(relattn_split_kernel<DP>, dim3((unsigned)total), dim3(256), 0, stream(), jobs);
@@ -1080,9 +1096,10 @@ static int run_forward(RelArgs& g) {
     g.splits = (int)ceil_div(g.sk > 0 ? g.sk : 1, g.keys_per_split);
     Scratch part, planes;
     if (g.splits > 1) {
-        if (!part.get(sizeof(float) * (size_t)(g.splits * rows) * (size_t)(g.d + 2))) return BH_ENOMEM;
-        g.part_o = (float*)part.p;
-        g.part_ml = g.part_o + (int64_t)g.splits * rows * g.d;
+        const int64_t ml = ceil_div(2 * g.splits * rows, 4) * 4;
+        if (!part.get(sizeof(float) * (size_t)(ml + g.splits * rows * g.d))) return BH_ENOMEM;
+        g.part_ml = (float*)part.p;
+        g.part_o = g.part_ml + ml;
     }
     int rc;
     if (by_rows) {
@@ -1117,21 +1134,23 @@ static int run_backward(RelArgs& g, float* dtable, int accumulate) {
     if (!delta.get(sizeof(float) * (size_t)rows) || !table.get(sizeof(double) * (size_t)wgs * (size_t)g.buckets)) return BH_ENOMEM;
     g.delta = (float*)delta.p;
     g.part_table = (double*)table.p;
-    hipLaunchKernelGGL(relattn_delta_kernel, dim3((unsigned)ceil_div(rows, 16)), dim3(256), 0, stream(), g);
-    int rc = BH_LAUNCH_CHECK("bh_relbias_attention_backward: delta");
-    if (rc) return rc;
-    if (g.sk > 0) {
+    int rc;
+    {
         g.k_blocks = (int)ceil_div(g.sk, 64) * 2;
         g.q_blocks = (int)ceil_div(g.sq, 32);
         const size_t kb = (size_t)g.batch * g.kv_heads * g.k_blocks * Block<DP>::BYTES, qb = (size_t)g.batch * g.heads * g.q_blocks * Block<DP>::BYTES;
-        if (!planes.get(3 * kb + 4 * qb)) return BH_ENOMEM;
+        if (!planes.get(3 * kb + 4 * qb)) return BH_ENOMEM;   // no keys: the planes of the queries alone are made, for the dots
         g.k_row = (const char*)planes.p; g.k_col = g.k_row + kb; g.v_row = g.k_col + kb;
         g.q_row = g.v_row + kb; g.q_col = g.q_row + qb; g.g_row = g.q_col + qb; g.g_col = g.g_row + qb;
         Planes p;
-        p.add(g.k, g.ks, g.kv_heads, g.batch, g.sk, g.kv_len, g.k_blocks, g.vec_k, g.k_row, g.k_col);
-        p.add(g.v, g.vs, g.kv_heads, g.batch, g.sk, g.kv_len, g.k_blocks, g.vec_v, g.v_row, nullptr);
+        if (g.sk > 0) {
+            p.add(g.k, g.ks, g.kv_heads, g.batch, g.sk, g.kv_len, g.k_blocks, g.vec_k, g.k_row, g.k_col);
+            p.add(g.v, g.vs, g.kv_heads, g.batch, g.sk, g.kv_len, g.k_blocks, g.vec_v, g.v_row, nullptr);
+        }
         p.add(g.q, g.qs, g.heads, g.batch, g.sq, nullptr, g.q_blocks, g.vec_q, g.q_row, g.q_col);
         p.add(g.d_out, g.os, g.heads, g.batch, g.sq, nullptr, g.q_blocks, g.vec_o, g.g_row, g.g_col);
+        p.last().with = g.out_in;
+        p.last().dots = g.delta;
         rc = p.launch<DP>(g.d);
         if (rc) return rc;
     }
