@@ -308,17 +308,13 @@ __device__ __forceinline__ int finish_scores(const RelArgs& g, const Bias& bias,
     return constant;
 }
 
-// workgroup number -> (batch*head, tile): the tiles of one head stay on one XCD, whose L2 then holds its keys and values;
-// tiles are numbered from the last (under a causal mask the longest) on
-__device__ __forceinline__ void head_and_tile(int id, int heads, int tiles, int& bh, int& tile) {
-    if (heads % kNumXcd == 0) {
-        bh = id % kNumXcd + kNumXcd * (id / kNumXcd / tiles);
-        tile = id / kNumXcd % tiles;
-    } else {
-        bh = id / tiles;
-        tile = id % tiles;
-    }
-    tile = tiles - 1 - tile;
+// workgroup number -> (batch*head, tile): a head's tiles stay on one XCD, whose L2 then holds its keys and values.  Tiles of one
+// length go head by head.  Under a causal mask (`falling`) all the heads' longest tiles (the last) come first and the shorter ones
+// fill up behind them: head by head the last head's longest tile would start when the others are nearly done.
+__device__ __forceinline__ void head_and_tile(int id, int heads, int tiles, bool falling, int& bh, int& tile) {
+    const int xcds = heads % kNumXcd == 0 ? kNumXcd : 1, x = id % xcds, j = id / xcds, per = heads / xcds;
+    bh = x + xcds * (falling ? j % per : j / tiles);
+    tile = tiles - 1 - (falling ? j / per : j % tiles);
 }
 
 constexpr int kThreads = 256, kWaves = 4, kQueryTile = 128;
@@ -396,13 +392,13 @@ template <int DP> struct ForwardLds {
 // A workgroup owns 128 queries of a head, a wavefront 32 of them, and walks over the keys.  Keys and values have a place in
 // LDS each: the next keys are on their way while the values are worked on and the other way round.
 template <int DP>
-__global__ __launch_bounds__(kThreads, 2) void relattn_forward_kernel(RelArgs g) {
+__global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : 2) void relattn_forward_kernel(RelArgs g) {
     using L = ForwardLds<DP>;
     constexpr int NB = L::NB, KEYS = 32 * NB, ND = DP / 32, KD = DP / 16;
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int bh, tile;
-    head_and_tile(blockIdx.x, g.batch * g.heads, g.q_tiles, bh, tile);
+    head_and_tile(blockIdx.x, g.batch * g.heads, g.q_tiles, g.causal, bh, tile);
     const int bt = bh / g.heads, h = bh % g.heads, hk = h / g.group;
     const float* q = g.q + bt * g.qs[0] + h * g.qs[1];
     const int64_t plane0 = ((int64_t)bt * g.kv_heads + hk) * g.k_blocks * Block<DP>::BYTES;
@@ -450,7 +446,7 @@ __global__ __launch_bounds__(kThreads, 2) void relattn_forward_kernel(RelArgs g)
             for (int b = 0; b < NB; b++) finish_scores(g, bias, s[b], c, k0 + 32 * b - rel_q, ke - k0 - 32 * b, wave, lane);
             running_softmax(s, m, l, o);
             u32x4 p[kPlanes];
-            pipelined<2 * NB * ND>([&](int i, u32x4 (&a)[kPlanes]) {
+            pipelined<2 * NB * ND, DP != 64>([&](int i, u32x4 (&a)[kPlanes]) {
                                        Block<DP>::column_fragment(smem + L::V + i / ND / 2 * Block<DP>::BYTES, i % ND, i / ND % 2, lane, a);
                                    },
                                    [&](int i, const u32x4 (&a)[kPlanes]) {
@@ -600,10 +596,15 @@ __global__ __launch_bounds__(256) void relattn_join_kernel(RelArgs g) {
     for (int c = lane; c < (g.d + 63) / 64 * 64; c += 64) {
         const float* p = g.part_o + row * g.d + min(c, g.d - 1);
         float a = 0.f;
-#pragma unroll 8
-        for (int s = 0; s < g.splits; s++) {
-            const float x = p[s * rows * g.d], y = __shfl(w, s, 64);
-            a += y == 0.f ? 0.f : y * x;
+        for (int s0 = 0; s0 < g.splits; s0 += 8) {                            // eight loads at a time; past the last split weight 0
+            float x[8];
+#pragma unroll
+            for (int s = 0; s < 8; s++) x[s] = p[min(s0 + s, g.splits - 1) * rows * g.d];
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                const float y = __shfl(w, s0 + s, 64);
+                a += y == 0.f ? 0.f : y * x[s];
+            }
         }
         if (c < g.d) dst[c] = a * f;
     }
@@ -632,7 +633,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
     double* sums = reinterpret_cast<double*>(smem + L::SUMS) + kMaxBuckets * wave;
     float* block = reinterpret_cast<float*>(smem + L::BLOCK) + 32 * 33 * wave;
     int bh, tile;
-    head_and_tile(blockIdx.x, g.batch * g.heads, g.q_tiles, bh, tile);
+    head_and_tile(blockIdx.x, g.batch * g.heads, g.q_tiles, g.causal, bh, tile);
     const int bt = bh / g.heads, h = bh % g.heads, hk = h / g.group;
     const float* q = g.q + bt * g.qs[0] + h * g.qs[1];
     const float* dout = g.d_out + bt * g.os[0] + h * g.os[1];
@@ -813,7 +814,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int bh, tile;
-    head_and_tile(blockIdx.x, g.batch * g.heads, k_tiles, bh, tile);
+    head_and_tile(blockIdx.x, g.batch * g.heads, k_tiles, g.causal, bh, tile);
     tile = k_tiles - 1 - tile;                                                // the first keys are seen by the most queries
     const int bt = bh / g.heads, h = bh % g.heads, hk = h / g.group;
     const float* k = g.k + bt * g.ks[0] + hk * g.ks[1];
