@@ -392,7 +392,7 @@ template <int DP> struct ForwardLds {
 // A workgroup owns 128 queries of a head, a wavefront 32 of them, and walks over the keys.  Keys and values have a place in
 // LDS each: the next keys are on their way while the values are worked on and the other way round.
 template <int DP>
-__global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : 2) void relattn_forward_kernel(RelArgs g) {
+__global__ __launch_bounds__(kThreads, 2) void relattn_forward_kernel(RelArgs g) {
     using L = ForwardLds<DP>;
     constexpr int NB = L::NB, KEYS = 32 * NB, ND = DP / 32, KD = DP / 16;
     extern __shared__ __align__(16) char smem[];
@@ -446,7 +446,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : 2) void relattn_forward_ke
             for (int b = 0; b < NB; b++) finish_scores(g, bias, s[b], c, k0 + 32 * b - rel_q, ke - k0 - 32 * b, wave, lane);
             running_softmax(s, m, l, o);
             u32x4 p[kPlanes];
-            pipelined<2 * NB * ND, DP != 64>([&](int i, u32x4 (&a)[kPlanes]) {
+            pipelined<2 * NB * ND>([&](int i, u32x4 (&a)[kPlanes]) {
                                        Block<DP>::column_fragment(smem + L::V + i / ND / 2 * Block<DP>::BYTES, i % ND, i / ND % 2, lane, a);
                                    },
                                    [&](int i, const u32x4 (&a)[kPlanes]) {
