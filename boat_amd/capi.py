@@ -40,6 +40,12 @@ class AttentionConfig(C.Structure):  # include/boat/layers/attention.h:21-30
                 ("use_rotary", C.c_bool), ("rotary_theta", C.c_float)]
 
 
+class RelativeAttentionConfig(C.Structure):
+    """boat_hip_relative_attention_config_t."""
+    _fields_ = [("num_buckets", C.c_int), ("max_distance", C.c_int), ("bidirectional", C.c_bool), ("causal", C.c_bool),
+                ("query_offset", C.c_int64), ("scale", C.c_float)]
+
+
 class LayerNormConfig(C.Structure):  # include/boat/layers/norm.h:21-26
     _fields_ = [("normalized_shape", C.c_size_t), ("eps", C.c_float),
                 ("elementwise_affine", C.c_bool), ("use_bias", C.c_bool)]
@@ -247,6 +253,12 @@ _EXT_SIGS = {
     "boat_hip_rmsnorm_get_weight": (P, [P]), "boat_hip_rmsnorm_get_grad_weight": (P, [P]),
     "boat_hip_softmax_cross_entropy": (P, [P, P, C.POINTER(P)]),
     "boat_hip_mse_loss": (P, [P, P, C.POINTER(P)]),
+    "boat_hip_dense_act": (P, [P, P, C.c_int, P, C.POINTER(P)]),
+    "boat_hip_var_dense_act": (P, [P, P, C.c_int, P]),
+    "boat_hip_relative_attention": (P, [C.POINTER(RelativeAttentionConfig), P, P, P, P, P, C.POINTER(P)]),
+    "boat_hip_var_relative_attention": (P, [C.POINTER(RelativeAttentionConfig), P, P, P, P, P]),
+    "boat_hip_distillation_loss": (P, [P, P, P, P, C.c_float, C.c_float, C.POINTER(P)]),
+    "boat_hip_var_distillation_loss": (P, [P, P, P, P, C.c_float, C.c_float]),
     "boat_hip_layer_from_dense": (P, [P]), "boat_hip_layer_from_norm": (P, [P]),
     "boat_hip_layer_relu": (P, []), "boat_hip_layer_gelu": (P, []),
     "boat_hip_optimizer_add_dense": (None, [P, P]),

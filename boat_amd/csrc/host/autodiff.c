@@ -22,16 +22,22 @@
 
 typedef enum {
     OP_ADD, OP_SUB, OP_MUL, OP_DIV, OP_RELU, OP_SIGMOID, OP_TANH, OP_MATMUL, OP_DOT, OP_SUM, OP_MEAN,
-    OP_SOFTMAX, OP_LOG_SOFTMAX, OP_FLATTEN, OP_DENSE, OP_ATTENTION, OP_GELU, OP_LAYERNORM, OP_CONV, OP_POOL
+    OP_SOFTMAX, OP_LOG_SOFTMAX, OP_FLATTEN, OP_DENSE, OP_ATTENTION, OP_GELU, OP_LAYERNORM, OP_CONV, OP_POOL,
+    OP_DENSE_ACT, OP_RELATIVE_ATTENTION, OP_DISTILLATION
 } op_type_t;
 
 typedef struct boat_op {
     op_type_t type;
-    boat_variable_t* inputs[3];
+    boat_variable_t* inputs[4];
     size_t num_inputs;
     boat_variable_t* output;     /* weak: the output owns the op */
     void* layer;                 /* dense / attention / layernorm */
-    boat_tensor_t* saved[3];     /* per-op saved tensors (layernorm: input, mean, rstd) */
+    boat_tensor_t* saved[6];     /* per-op saved tensors (layernorm: input, mean, rstd) */
+    union {
+        int act;                                             /* OP_DENSE_ACT */
+        boat_hip_relative_attention_config_t relative;       /* OP_RELATIVE_ATTENTION */
+        struct { float temperature, alpha; } distillation;   /* OP_DISTILLATION */
+    } how;
     uint64_t seq;                /* recording order == a topological order */
     uint64_t mark;               /* visit epoch of the backward that last collected it */
     uint64_t skip;               /* visit epoch of a backward in which a fused rule already covered this op */
@@ -87,7 +93,7 @@ static void variable_unref(boat_variable_t* v);
 
 static void op_free(boat_op_t* op) {
     if (!op) return;
-    for (size_t i = 0; i < 3; i++) boat_tensor_free(op->saved[i]);
+    for (size_t i = 0; i < sizeof(op->saved) / sizeof(op->saved[0]); i++) boat_tensor_free(op->saved[i]);
     for (size_t i = 0; i < op->num_inputs; i++) variable_unref(op->inputs[i]);
     free(op);
 }
@@ -377,6 +383,66 @@ boat_variable_t* boat_hip_var_layernorm(const boat_variable_t* a, boat_layernorm
         op->saved[2] = norm->cache_rstd;
         for (int i = 0; i < 3; i++) boat_tensor_ref(op->saved[i]);
     }
+    return out;
+}
+
+/* The fused operators keep references to the tensors their backward pass reads: a variable's data may be reset before it. */
+static void keep(boat_op_t* op, int slot, const boat_tensor_t* t) {
+    op->saved[slot] = (boat_tensor_t*)t;
+    if (t) boat_tensor_ref(op->saved[slot]);
+}
+
+boat_variable_t* boat_hip_var_dense_act(const boat_variable_t* input, boat_dense_layer_t* layer, boat_hip_activation_t act,
+                                        const boat_variable_t* residual) {
+    if (!input || !layer) return NULL;
+    boat_variable_t* in[2] = {(boat_variable_t*)input, (boat_variable_t*)residual};
+    const bool grad = input->requires_grad || (residual && residual->requires_grad);
+    boat_tensor_t* saved = NULL;
+    boat_tensor_t* y = boat_hip_dense_act(layer, input->data, act, residual ? residual->data : NULL, grad && recording() ? &saved : NULL);
+    boat_variable_t* out = record(OP_DENSE_ACT, in, residual ? 2 : 1, y, grad, layer);
+    if (out && out->producer) {
+        keep(out->producer, 0, input->data);
+        keep(out->producer, 1, saved);
+        out->producer->how.act = (int)act;
+    }
+    boat_tensor_free(saved);
+    return out;
+}
+
+boat_variable_t* boat_hip_var_relative_attention(const boat_hip_relative_attention_config_t* config, const boat_variable_t* query,
+                                                 const boat_variable_t* key, const boat_variable_t* value,
+                                                 const boat_variable_t* table, const boat_tensor_t* lengths) {
+    if (!config || !query || !key || !value || !table) return NULL;
+    boat_variable_t* in[4] = {(boat_variable_t*)query, (boat_variable_t*)key, (boat_variable_t*)value, (boat_variable_t*)table};
+    const bool grad = query->requires_grad || key->requires_grad || value->requires_grad || table->requires_grad;
+    boat_tensor_t* lse = NULL;
+    boat_tensor_t* y = boat_hip_relative_attention(config, query->data, key->data, value->data, table->data, lengths, &lse);
+    boat_variable_t* out = record(OP_RELATIVE_ATTENTION, in, 4, y, grad, NULL);
+    if (out && out->producer) {
+        for (int i = 0; i < 4; i++) keep(out->producer, i, in[i]->data);
+        keep(out->producer, 4, lse);
+        keep(out->producer, 5, lengths);
+        out->producer->how.relative = *config;
+    }
+    boat_tensor_free(lse);
+    return out;
+}
+
+boat_variable_t* boat_hip_var_distillation_loss(const boat_variable_t* logits, const boat_tensor_t* teacher, const boat_tensor_t* index,
+                                                const boat_tensor_t* labels, float temperature, float alpha) {
+    if (!logits || !teacher || !index) return NULL;
+    boat_variable_t* in[1] = {(boat_variable_t*)logits};
+    boat_tensor_t* stats = NULL;
+    boat_tensor_t* y = bt_distillation_forward(logits->data, teacher, index, labels, temperature, alpha,
+                                               logits->requires_grad && recording() ? &stats : NULL);
+    boat_variable_t* out = record(OP_DISTILLATION, in, 1, y, logits->requires_grad, NULL);
+    if (out && out->producer) {
+        const boat_tensor_t* kept[5] = {logits->data, teacher, index, labels, stats};
+        for (int i = 0; i < 5; i++) keep(out->producer, i, kept[i]);
+        out->producer->how.distillation.temperature = temperature;
+        out->producer->how.distillation.alpha = alpha;
+    }
+    boat_tensor_free(stats);
     return out;
 }
 
@@ -679,6 +745,31 @@ static void backward_op(boat_op_t* op, const boat_tensor_t* dy) {
             }
             break;
         }
+        case OP_DENSE_ACT: {
+            boat_tensor_t* dx = NULL;
+            /* the residual was added last: its gradient is dy itself */
+            if (b && b->requires_grad) accumulate(b, (boat_tensor_t*)dy, false);
+            if (bt_dense_act_backward((boat_dense_layer_t*)op->layer, op->how.act, op->saved[0], op->saved[1], dy,
+                                      a->requires_grad ? &dx : NULL) && dx)
+                accumulate(a, dx, true);
+            break;
+        }
+        case OP_RELATIVE_ATTENTION: {
+            boat_tensor_t* g[4];
+            if (!bt_relative_attention_backward(&op->how.relative, op->saved[0], op->saved[1], op->saved[2], op->saved[3], op->saved[5],
+                                                op->output->data, op->saved[4], dy, g))
+                break;
+            for (int i = 0; i < 4; i++) {
+                if (op->inputs[i]->requires_grad) accumulate(op->inputs[i], g[i], true);
+                else boat_tensor_free(g[i]);
+            }
+            break;
+        }
+        case OP_DISTILLATION:
+            if (a->requires_grad)
+                accumulate(a, bt_distillation_backward(op->saved[0], op->saved[1], op->saved[2], op->saved[3], op->how.distillation.temperature,
+                                                       op->how.distillation.alpha, op->saved[4], dy), true);
+            break;
     }
 }
 
@@ -844,7 +935,8 @@ void boat_autodiff_set_grad_checkpointing(bool enabled) { (void)enabled; }
 
 static const char* op_name(op_type_t t) {
     static const char* names[] = {"add", "sub", "mul", "div", "relu", "sigmoid", "tanh", "matmul", "dot", "sum", "mean",
-                                  "softmax", "log_softmax", "flatten", "dense", "attention", "gelu", "layernorm", "conv", "pool"};
+                                  "softmax", "log_softmax", "flatten", "dense", "attention", "gelu", "layernorm", "conv", "pool",
+                                  "dense_act", "relative_attention", "distillation"};
     return (size_t)t < sizeof(names) / sizeof(names[0]) ? names[t] : "?";
 }
 

@@ -151,6 +151,18 @@ boat_tensor_t* bt_dense_layer_backward_bias_done(boat_dense_layer_t* layer, cons
 /* where a rule that computes this layer's grad_output [rows, cols] may add that call's bias gradient itself: the device
  * pointer of grad_bias and whether to add or to write (NULL: the layer has no bias of that width; nothing is touched) */
 float* bt_dense_bias_grad_target(boat_dense_layer_t* layer, int64_t cols, int* accumulate);
+/* fused.c: the forward and backward passes behind the boat_hip_dense_act, _relative_attention and _distillation_loss pairs */
+bool bt_dense_act_backward(boat_dense_layer_t* layer, int act, const boat_tensor_t* input, const boat_tensor_t* saved,
+                           const boat_tensor_t* dy, boat_tensor_t** dx);
+bool bt_relative_attention_backward(const boat_hip_relative_attention_config_t* config, const boat_tensor_t* query,
+                                    const boat_tensor_t* key, const boat_tensor_t* value, const boat_tensor_t* table,
+                                    const boat_tensor_t* lengths, const boat_tensor_t* out, const boat_tensor_t* lse,
+                                    const boat_tensor_t* dy, boat_tensor_t* grads[4]);
+boat_tensor_t* bt_distillation_forward(const boat_tensor_t* logits, const boat_tensor_t* teacher, const boat_tensor_t* index,
+                                       const boat_tensor_t* labels, float temperature, float alpha, boat_tensor_t** stats);
+boat_tensor_t* bt_distillation_backward(const boat_tensor_t* logits, const boat_tensor_t* teacher, const boat_tensor_t* index,
+                                        const boat_tensor_t* labels, float temperature, float alpha, const boat_tensor_t* stats,
+                                        const boat_tensor_t* dy);
 boat_tensor_t* boat_layernorm_backward_add_impl(boat_layernorm_t* norm, const boat_tensor_t* x, const boat_tensor_t* mean,
                                                 const boat_tensor_t* rstd, const boat_tensor_t* grad_output, const boat_tensor_t* add);
 

@@ -443,6 +443,53 @@ static void tour_norms_attention_core_and_types(void) {
     boat_hip_set_reference_exact(0);
 }
 
+/* ---- a student's block and its loss: dense with activation and residual, relative attention, distillation ---- */
+static void tour_student(void) {
+    enum { B = 2, S = 5, H = 2, D = 8, W = H * D, V = 11, KEPT = 3, BUCKETS = 8 };
+    const int64_t flat[2] = {B * S, W}, split[4] = {B, S, H, D}, ts[2] = {BUCKETS, H}, ks[2] = {B * S, KEPT}, rs[1] = {B * S}, bs[1] = {B};
+    boat_tensor_t* x = random_tensor(flat, 2, 1.0f);
+    boat_tensor_t* bias = random_tensor(ts, 2, 1.0f);
+    boat_tensor_t* teacher = random_tensor(ks, 2, 3.0f);
+    boat_tensor_t* index = boat_tensor_create(ks, 2, BOAT_DTYPE_INT32, BOAT_DEVICE_CPU);
+    boat_tensor_t* labels = boat_tensor_create(rs, 1, BOAT_DTYPE_INT32, BOAT_DEVICE_CPU);
+    boat_tensor_t* lengths = boat_tensor_create(bs, 1, BOAT_DTYPE_INT32, BOAT_DEVICE_CPU);
+    for (int i = 0; i < B * S * KEPT; i++) ((int32_t*)boat_tensor_data(index))[i] = (i * 5) % V;
+    for (int i = 0; i < B * S; i++) ((int32_t*)boat_tensor_data(labels))[i] = i % V;
+    for (int i = 0; i < B; i++) ((int32_t*)boat_tensor_data(lengths))[i] = S - i;
+    boat_dense_layer_t* in = boat_dense_layer_create(W, W, true);
+    boat_dense_layer_t* mix = boat_dense_layer_create(W, W, true);
+    boat_dense_layer_t* head = boat_dense_layer_create(W, V, false);
+    const boat_hip_relative_attention_config_t config = {BUCKETS, 16, true, false, 0, 0.35f};
+    boat_variable_t* vx = boat_variable_create(x, true);
+    boat_variable_t* vt = boat_variable_create(bias, true);
+    boat_variable_t* h = boat_hip_var_dense_act(vx, in, BOAT_HIP_ACT_GELU, NULL);
+    boat_variable_t* h4 = boat_hip_var_reshape(h, split, 4);
+    boat_variable_t* a4 = boat_hip_var_relative_attention(&config, h4, h4, h4, vt, lengths);
+    boat_variable_t* a = boat_hip_var_reshape(a4, flat, 2);
+    boat_variable_t* y = boat_hip_var_dense_act(a, mix, BOAT_HIP_ACT_TANH, vx);
+    boat_variable_t* z = boat_hip_var_dense_act(y, head, BOAT_HIP_ACT_NONE, NULL);
+    boat_variable_t* loss = boat_hip_var_distillation_loss(z, teacher, index, labels, 2.0f, 0.5f);
+    CHECK(loss && isfinite(first_value(boat_variable_data(loss))));
+    boat_variable_backward_full(loss);
+    CHECK(boat_variable_grad(vx) && isfinite(sum_abs(boat_variable_grad(vx))) && sum_abs(boat_variable_grad(vx)) > 0.0f);
+    CHECK(boat_variable_grad(vt) && sum_abs(boat_variable_grad(vt)) > 0.0f);
+    /* the eager forms give the tape's values */
+    boat_tensor_t *dz = NULL, *lse = NULL, *saved = NULL;
+    boat_tensor_t* eager = boat_hip_distillation_loss(boat_variable_data(z), teacher, index, labels, 2.0f, 0.5f, &dz);
+    boat_tensor_t* attended = boat_hip_relative_attention(&config, boat_variable_data(h4), boat_variable_data(h4), boat_variable_data(h4), bias, lengths, &lse);
+    boat_tensor_t* dense = boat_hip_dense_act(mix, boat_variable_data(a), BOAT_HIP_ACT_TANH, x, &saved);
+    CHECK(eager && dz && fabsf(first_value(eager) - first_value(boat_variable_data(loss))) <= 1e-5f * fabsf(first_value(eager)));
+    CHECK(attended && lse && sum_abs(attended) == sum_abs(boat_variable_data(a4)));
+    CHECK(dense && saved && sum_abs(dense) == sum_abs(boat_variable_data(y)));
+    boat_variable_t* vars[] = {loss, z, y, a, a4, h4, h, vt, vx};
+    for (size_t i = 0; i < sizeof(vars) / sizeof(vars[0]); i++) boat_variable_free(vars[i]);
+    boat_tensor_t* tensors[] = {dense, saved, attended, lse, eager, dz, lengths, labels, index, teacher, bias, x};
+    for (size_t i = 0; i < sizeof(tensors) / sizeof(tensors[0]); i++) boat_tensor_unref(tensors[i]);
+    boat_dense_layer_free(head);
+    boat_dense_layer_free(mix);
+    boat_dense_layer_free(in);
+}
+
 int main(void) {
     boat_init();
     if (boat_has_error()) {
@@ -454,6 +501,7 @@ int main(void) {
     tour_layers();
     tour_attention_and_conv();
     tour_norms_attention_core_and_types();
+    tour_student();
     boat_hip_synchronize();
     CHECK(!boat_has_error());
     const boat_memory_stats_t st = boat_memory_get_stats();

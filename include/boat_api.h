@@ -497,6 +497,48 @@ BOAT_API boat_tensor_t* boat_hip_rmsnorm_get_grad_weight(const boat_rmsnorm_t* n
 BOAT_API boat_tensor_t* boat_hip_softmax_cross_entropy(const boat_tensor_t* logits, const boat_tensor_t* labels, boat_tensor_t** dlogits);
 /* mean squared error (src/loss/mse.c:70-78) and its gradient 2(o-t)/n (tests/test_attention_training.c:28-41) */
 BOAT_API boat_tensor_t* boat_hip_mse_loss(const boat_tensor_t* pred, const boat_tensor_t* target, boat_tensor_t** grad);
+/* ---- pieces of a small model trained against a large one's answers ----
+ * A dense layer that finishes its block in one kernel: act(input . W + bias) + residual.  input [rows, in], residual
+ * [rows, out] or NULL.  *saved (may be NULL) receives what the backward pass needs, a reference the caller frees; the two
+ * forms record nothing in the layer.  With gradients tracked the layer's weight and bias gradients accumulate as
+ * boat_var_dense's do; recorded when the input or the residual requires a gradient. */
+typedef enum {
+    BOAT_HIP_ACT_NONE = -1, BOAT_HIP_ACT_RELU, BOAT_HIP_ACT_SIGMOID, BOAT_HIP_ACT_TANH, BOAT_HIP_ACT_GELU
+} boat_hip_activation_t;
+BOAT_API boat_tensor_t* boat_hip_dense_act(const boat_dense_layer_t* layer, const boat_tensor_t* input, boat_hip_activation_t act,
+                                           const boat_tensor_t* residual, boat_tensor_t** saved);
+BOAT_API boat_variable_t* boat_hip_var_dense_act(const boat_variable_t* input, boat_dense_layer_t* layer,
+                                                 boat_hip_activation_t act, const boat_variable_t* residual);
+/* Attention with a learned bias per bucket of relative positions: softmax(scale q.k + table[bucket(key - query)][head]) v.
+ * query [batch, seq_q, heads, head_size]; key and value [batch, seq_k, kv_heads, head_size], heads a multiple of kv_heads
+ * (neighbouring heads share a key head); table [num_buckets, heads]; lengths: NULL or INT32 [batch], the number of valid
+ * keys of each sequence.  head_size at most 128.  So the [batch*seq, heads*head_size] output of a dense layer is reshaped,
+ * never transposed.  Returns the shape of query; *lse (may be NULL) receives the [batch, heads, seq_q] row log-sum-exp.
+ * query_offset: position of the first query counted from the first key (seq_k - seq_q for the last tokens of a sequence). */
+typedef struct {
+    int num_buckets, max_distance;
+    bool bidirectional;          /* half of the buckets for keys behind the query, half for keys ahead */
+    bool causal;
+    int64_t query_offset;
+    float scale;
+} boat_hip_relative_attention_config_t;
+BOAT_API boat_tensor_t* boat_hip_relative_attention(const boat_hip_relative_attention_config_t* config, const boat_tensor_t* query,
+                                                    const boat_tensor_t* key, const boat_tensor_t* value,
+                                                    const boat_tensor_t* table, const boat_tensor_t* lengths, boat_tensor_t** lse);
+BOAT_API boat_variable_t* boat_hip_var_relative_attention(const boat_hip_relative_attention_config_t* config,
+                                                          const boat_variable_t* query, const boat_variable_t* key,
+                                                          const boat_variable_t* value, const boat_variable_t* table,
+                                                          const boat_tensor_t* lengths);
+/* Mean over the rows of alpha T^2 KL(teacher || student) at temperature T over the teacher's kept logits + (1 - alpha) cross
+ * entropy with the label.  logits [rows, vocab]; teacher (float) and index (INT32) [rows, kept]; labels: NULL or INT32
+ * [rows].  Indices and labels outside the vocabulary leave their entry out.  Returns the [1] loss and, through *dlogits (may
+ * be NULL), its gradient; the second form records it. */
+BOAT_API boat_tensor_t* boat_hip_distillation_loss(const boat_tensor_t* logits, const boat_tensor_t* teacher, const boat_tensor_t* index,
+                                                   const boat_tensor_t* labels, float temperature, float alpha, boat_tensor_t** dlogits);
+BOAT_API boat_variable_t* boat_hip_var_distillation_loss(const boat_variable_t* logits, const boat_tensor_t* teacher,
+                                                         const boat_tensor_t* index, const boat_tensor_t* labels,
+                                                         float temperature, float alpha);
+
 /* ready-made vtables for boat_model_add_layer (the reference ships none; callers write these wrappers,
  * tests/test_model_graph_integration.c:8-77).  The returned boat_layer_t is freed by ops->free. */
 BOAT_API boat_layer_t* boat_hip_layer_from_dense(boat_dense_layer_t* layer);
