@@ -47,14 +47,16 @@ struct RelArgs {
     int causal;
     float scale;
     bool vec_q, vec_k, vec_v, vec_o;
-    int splits; int64_t keys_per_split;    // forward over few workgroups: partial results per split
+    int splits; int64_t keys_per_split;    // few workgroups (forward, dQ): partial results per split of the keys
     float *part_o, *part_ml;               // [split][batch*heads*sq][d], [split][batch*heads*sq][2]
     float* delta;                          // backward: rowsum(dO o O)
-    double* part_table;                    // backward: [batch*heads][query tiles][buckets]
+    double* part_table;                    // backward: [split][batch*heads][query tiles][buckets]
     int buckets, q_tiles;
     const char *k_row, *k_col, *v_row, *v_col, *q_row, *q_col, *g_row, *g_col;   // planes
     int k_blocks, q_blocks;                // of 32 rows, per head
-    float *part_k, *part_v;                // backward, shared key heads: [batch*heads][sk][d]
+    float* part_q;                         // backward over split keys: [split][batch*heads][sq][d]
+    int q_splits, queries_per_split;       // dK, dV: splits of the queries
+    float *part_k, *part_v;                // shared key heads or split queries: [split][batch*heads][sk][d]
     Buckets b;
 };
 
@@ -428,7 +430,9 @@ __global__ __launch_bounds__(kThreads, 2) void relattn_forward_kernel(RelArgs g)
     float m = -INFINITY, l = 0.f;
     const float c = g.scale * kLog2e;
     wait_copies();
-    for (int k0 = kb; k0 < ke; k0 += KEYS) {
+    int k0 = kb;
+    asm volatile("" : "+s"(k0));                                              // keeps the fragments' making apart from the steps
+    for (; k0 < ke; k0 += KEYS) {
         copy_to_lds<2 * NB * DP * 96 / 1024, kWaves>(vp + (int64_t)(k0 / 32) * Block<DP>::BYTES, smem + L::V, wave, lane);
         const bool mine = qw < g.sq && !(g.causal && k0 > rel_q + 31);        // else nothing here for this wavefront
         f32x16 s[NB];
@@ -646,13 +650,15 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
     const int len = g.kv_len ? min(max(g.kv_len[bt], 0), (int)g.sk) : (int)g.sk;
     int ke = len;
     if (g.causal) ke = (int)min((int64_t)ke, max((int64_t)0, min((int64_t)q0 + kQueryTile, g.sq) + g.offset));
+    const int kb = (int)(blockIdx.y * g.keys_per_split);
+    ke = (int)min((int64_t)ke, kb + g.keys_per_split);
     const int rel_q = (int)(qw + g.offset);
     const auto fetch_rows = [&](int k0) {
         const int64_t at = plane0 + (int64_t)(k0 / 32) * Block<DP>::BYTES;
         copy_to_lds<KB, kWaves>(g.k_row + at, smem, wave, lane);
         copy_to_lds<KB, kWaves>(g.v_row + at, smem + L::V, wave, lane);
     };
-    if (ke > 0) fetch_rows(0);
+    if (kb < ke) fetch_rows(kb);
     // The matrix cores' sums are cut towards minus infinity by some hundredths of a step.  For one element that is nothing, but
     // the table's gradient adds up a million of them that nearly cancel: odd queries are negated, and their results again, so
     // that the cuts cancel too (8 x 16 heads x 1024 x 1024: the table's relative error 4e-6 without, 4e-7 with it).
@@ -680,7 +686,9 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
     // A bucket's sum is small against its terms (a row of dS adds up to zero): blocks are added up in 64 bits
     double far_sum[2] = {0.0, 0.0};                                           // blocks that lie in one bucket: before, behind
     wait_copies();
-    for (int k0 = 0; k0 < ke; k0 += KEYS) {
+    int k0 = kb;
+    asm volatile("" : "+s"(k0));                                              // keeps the fragments' making apart from the steps
+    for (; k0 < ke; k0 += KEYS) {
         copy_to_lds<KB, kWaves>(g.k_col + plane0 + (int64_t)(k0 / 32) * Block<DP>::BYTES, smem + L::KT, wave, lane);
         const bool mine = qw < g.sq && !(g.causal && k0 > rel_q + 31);
         f32x16 s, dp;
@@ -755,11 +763,13 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
     }
     __syncthreads();
     const double* all = reinterpret_cast<const double*>(smem + L::SUMS);
+    const int64_t split_bh = (int64_t)blockIdx.y * g.batch * g.heads;
     for (int i = tid; i < g.buckets; i += kThreads)
-        g.part_table[((int64_t)bh * g.q_tiles + tile) * g.buckets + i] =
+        g.part_table[((split_bh + bh) * g.q_tiles + tile) * g.buckets + i] =
             (all[i] + all[kMaxBuckets + i]) + (all[2 * kMaxBuckets + i] + all[3 * kMaxBuckets + i]);
     if (!live) return;
-    float* dst = g.dq + bt * g.qs[0] + h * g.qs[1] + qi * g.qs[2];
+    const bool part = g.splits > 1, vec = part ? g.d % 4 == 0 : g.vec_q;
+    float* dst = part ? g.part_q + ((split_bh + bh) * g.sq + qi) * g.d : g.dq + bt * g.qs[0] + h * g.qs[1] + qi * g.qs[2];
 #pragma unroll
     for (int b = 0; b < DP / 32; b++)
 #pragma unroll
@@ -768,33 +778,12 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
             f32x4 y;
 #pragma unroll
             for (int j = 0; j < 4; j++) y[j] = dq[b][e + j] * g.scale;
-            if (g.vec_q && cd + 4 <= g.d) *reinterpret_cast<f32x4*>(dst + cd) = y;
+            if (vec && cd + 4 <= g.d) *reinterpret_cast<f32x4*>(dst + cd) = y;
             else
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     if (cd + j < g.d) dst[cd + j] = y[j];
         }
-}
-
-// dT: the workgroups' parts of a head, over batch and tiles in order
-__global__ __launch_bounds__(256) void relattn_table_kernel(RelArgs g, float* __restrict__ dtable, int accumulate) {
-    __shared__ double red[256];
-    const int h = blockIdx.y, b0 = blockIdx.x * 16, b = b0 + (threadIdx.x & 15), part = threadIdx.x >> 4;
-    double s = 0.0;
-    const int total = g.batch * g.q_tiles;
-    if (b < g.buckets)
-        for (int i = part; i < total; i += 16) {
-            const int64_t bh = (int64_t)(i / g.q_tiles) * g.heads + h;
-            s += g.part_table[(bh * g.q_tiles + i % g.q_tiles) * g.buckets + b];
-        }
-    red[threadIdx.x] = s;
-    __syncthreads();
-    if (threadIdx.x < 16 && b < g.buckets) {
-        double t = 0.0;
-        for (int i = 0; i < 16; i++) t += red[i * 16 + threadIdx.x];
-        float* dst = dtable + (int64_t)b * g.heads + h;
-        *dst = accumulate ? *dst + (float)t : (float)t;
-    }
 }
 
 template <int DP> struct KeyLds {
@@ -808,12 +797,13 @@ template <int DP> struct KeyLds {
 // dK and dV of one query head: a workgroup owns 128 keys and walks over the queries.  Heads that share a key head leave their
 // parts in work memory (one long chain of sums over all of them would round more, and fill fewer compute units)
 template <int DP>
-__global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel(RelArgs g, int k_tiles) {
+__global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel(RelArgs g) {
     using L = KeyLds<DP>;
     constexpr int ROWS = 32, ND = DP / 32, KD = DP / 16, KB = Block<DP>::BYTES / 1024;
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int bh, tile;
+    const int k_tiles = (int)((g.sk + 127) / 128);
     head_and_tile(blockIdx.x, g.batch * g.heads, k_tiles, g.causal, bh, tile);
     tile = k_tiles - 1 - tile;                                                // the first keys are seen by the most queries
     const int bt = bh / g.heads, h = bh % g.heads, hk = h / g.group;
@@ -837,12 +827,14 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
     const float c = g.scale * kLog2e;
     int qb = 0;                                                               // causal: the first query that sees a key of the workgroup
     if (g.causal) qb = (int)(min((int64_t)sq, max((int64_t)0, (int64_t)tile * 128 - g.offset)) / ROWS * ROWS);
+    const int qe = min(sq, (int)(blockIdx.y + 1) * g.queries_per_split);
+    qb = max(qb, (int)blockIdx.y * g.queries_per_split);
     if (tile * 128 >= len) qb = sq;                                           // only padding here
     // One turn of a loop that the compiler cannot see to be one: it then keeps the fragments' making apart from the steps.
     // Run together they need 47 registers more than there are at head size 128.
     int turns = 1;
     asm volatile("" : "+s"(turns));
-    for (; turns > 0 && qb < sq; turns--) {
+    for (; turns > 0 && qb < qe; turns--) {
         const int64_t row0 = (int64_t)bh * g.sq, plane0 = (int64_t)bh * g.q_blocks * Block<DP>::BYTES;
         const auto fetch = [&](const char* q, const char* d, int r0, int at) {
             const int64_t o = plane0 + (int64_t)(r0 / 32) * Block<DP>::BYTES;
@@ -858,7 +850,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
         const Bias bias(g, h, smem + L::BIAS, kThreads);
         // from the last queries down: under a causal mask, where the key tiles have different first queries, all the workgroups
         // of a head are then at the same queries at the same time and read them out of the L2 once
-        const int q_last = (sq - 1) / ROWS * ROWS;
+        const int q_last = (qe - 1) / ROWS * ROWS;
         fetch(g.q_row, g.g_row, q_last, 0);
         fetch_stat(q_last, 0);
         wait_copies();
@@ -923,11 +915,11 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
         }
     }
     if (ki >= g.sk) return;
-    const bool shared = g.group > 1;
-    const int64_t at = ((int64_t)bh * g.sk + ki) * g.d;
-    float* pk = shared ? g.part_k + at : g.dk + bt * g.ks[0] + hk * g.ks[1] + ki * g.ks[2];
-    float* pv = shared ? g.part_v + at : g.dv + bt * g.vs[0] + hk * g.vs[1] + ki * g.vs[2];
-    const bool vec_k = shared ? g.d % 4 == 0 : g.vec_k, vec_v = shared ? g.d % 4 == 0 : g.vec_v;
+    const bool part = g.part_k;
+    const int64_t at = (((int64_t)blockIdx.y * g.batch * g.heads + bh) * g.sk + ki) * g.d;
+    float* pk = part ? g.part_k + at : g.dk + bt * g.ks[0] + hk * g.ks[1] + ki * g.ks[2];
+    float* pv = part ? g.part_v + at : g.dv + bt * g.vs[0] + hk * g.vs[1] + ki * g.vs[2];
+    const bool vec_k = part ? g.d % 4 == 0 : g.vec_k, vec_v = part ? g.d % 4 == 0 : g.vec_v;
 #pragma unroll
     for (int b = 0; b < ND; b++)
 #pragma unroll
@@ -950,16 +942,48 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
         }
 }
 
-// the parts of the heads that share a key head, in order
-__global__ __launch_bounds__(256) void relattn_heads_kernel(RelArgs g) {
-    const int64_t per = g.sk * g.d, total = (int64_t)g.batch * g.kv_heads * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t bk = i / per, at = i - bk * per, row = at / g.d, c = at - row * g.d, bt = bk / g.kv_heads, hk = bk - bt * g.kv_heads;
-        const int64_t first = (bt * g.heads + hk * g.group) * per + at;
-        float x = g.part_k[first], y = g.part_v[first];
-        for (int h = 1; h < g.group; h++) { x += g.part_k[first + h * per]; y += g.part_v[first + h * per]; }
-        g.dk[bt * g.ks[0] + hk * g.ks[1] + row * g.ks[2] + c] = x;
-        g.dv[bt * g.vs[0] + hk * g.vs[1] + row * g.vs[2] + c] = y;
+// What is left in parts, added up in order: the first workgroups make dT (16 buckets of a head each, over splits, batch and
+// tiles), the next ones dQ where the keys were split, the last ones dK and dV where the queries were or heads share a key head.
+struct Fold { int table_blocks, q_blocks, k_blocks; float* dtable; int accumulate; };
+__global__ __launch_bounds__(256) void relattn_fold_kernel(RelArgs g, Fold f) {
+    __shared__ double red[256];
+    const int id = blockIdx.x;
+    if (id < f.table_blocks) {
+        const int h = id % g.heads, b = id / g.heads * 16 + (threadIdx.x & 15), first = threadIdx.x >> 4;
+        const int64_t total = (int64_t)g.splits * g.batch * g.q_tiles;
+        double s = 0.0;
+        if (b < g.buckets)
+            for (int64_t i = first; i < total; i += 16) {
+                const int64_t bt = i / g.q_tiles, bh = bt * g.heads + h;
+                s += g.part_table[(bh * g.q_tiles + (i - bt * g.q_tiles)) * g.buckets + b];
+            }
+        red[threadIdx.x] = s;
+        __syncthreads();
+        if (threadIdx.x < 16 && b < g.buckets) {
+            double t = 0.0;
+            for (int i = 0; i < 16; i++) t += red[i * 16 + threadIdx.x];
+            float* dst = f.dtable + (int64_t)b * g.heads + h;
+            *dst = f.accumulate ? *dst + (float)t : (float)t;
+        }
+    } else if (id < f.table_blocks + f.q_blocks) {
+        const int64_t per = g.sq * g.d, total = (int64_t)g.batch * g.heads * per;
+        for (int64_t i = (int64_t)(id - f.table_blocks) * 256 + threadIdx.x; i < total; i += (int64_t)f.q_blocks * 256) {
+            const int64_t bh = i / per, at = i - bh * per, row = at / g.d, c = at - row * g.d, bt = bh / g.heads, h = bh - bt * g.heads;
+            float x = g.part_q[i];
+            for (int p = 1; p < g.splits; p++) x += g.part_q[i + p * total];
+            g.dq[bt * g.qs[0] + h * g.qs[1] + row * g.qs[2] + c] = x;
+        }
+    } else {
+        const int64_t per = g.sk * g.d, total = (int64_t)g.batch * g.kv_heads * per, all = (int64_t)g.batch * g.heads * per;
+        for (int64_t i = (int64_t)(id - f.table_blocks - f.q_blocks) * 256 + threadIdx.x; i < total; i += (int64_t)f.k_blocks * 256) {
+            const int64_t bk = i / per, at = i - bk * per, row = at / g.d, c = at - row * g.d, bt = bk / g.kv_heads, hk = bk - bt * g.kv_heads;
+            const int64_t first = (bt * g.heads + hk * g.group) * per + at;
+            float x = 0.f, y = 0.f;
+            for (int p = 0; p < g.q_splits; p++)
+                for (int h = 0; h < g.group; h++) { x += g.part_k[first + h * per + p * all]; y += g.part_v[first + h * per + p * all]; }
+            g.dk[bt * g.ks[0] + hk * g.ks[1] + row * g.ks[2] + c] = x;
+            g.dv[bt * g.vs[0] + hk * g.vs[1] + row * g.vs[2] + c] = y;
+        }
     }
 }
 
@@ -999,6 +1023,8 @@ static bool vectors(const void* p, const int64_t (&s)[3], int d) {
     return aligned16(p) && d % 4 == 0 && s[0] % 4 == 0 && s[1] % 4 == 0 && s[2] % 4 == 0;
 }
 
+constexpr int64_t kMostGroups = (1 << 23) - 1;            // workgroups of one launch: their threads are counted in 32 bits
+
 static int relattn_args(const char* fn, const bh_relbias_attention_t* p, RelArgs& g) {
     if (!p) return set_error(BH_EINVAL, "%s: null pointer", fn);
     if (p->batch < 0 || p->heads < 0 || p->kv_heads < 0 || p->sq < 0 || p->sk < 0) return set_error(BH_EINVAL, "%s: negative dimension", fn);
@@ -1007,7 +1033,7 @@ static int relattn_args(const char* fn, const bh_relbias_attention_t* p, RelArgs
     const int64_t most = (int64_t)1 << 28;                // sums and differences of them stay within 32 bits
     if (p->sq > most || p->sk > most || p->query_offset > most || p->query_offset < -most)
         return set_error(BH_EINVAL, "%s: sequences and offset are at most 2^28", fn);
-    if (p->batch * p->heads > 0x7fffffff / 2 || p->batch > 0x7fffffff || p->heads > 0x7fffffff) return set_error(BH_EINVAL, "%s: too many heads", fn);
+    if (p->batch > 0x7fffffff || p->heads > 0x7fffffff || p->batch * p->heads > 0x7fffffff / 2) return set_error(BH_EINVAL, "%s: too many heads", fn);
     if (p->batch * p->heads > 0 && (ceil_div(p->sq, 32) > 0x3fffffff / (p->batch * p->heads) || ceil_div(p->sk, 32) > 0x3fffffff / (p->batch * p->heads)))
         return set_error(BH_EINVAL, "%s: too many rows", fn);
     for (int i = 0; i < 3; i++)
@@ -1022,7 +1048,9 @@ static int relattn_args(const char* fn, const bh_relbias_attention_t* p, RelArgs
     for (int i = 0; i < 3; i++) { g.qs[i] = p->q_stride[i]; g.ks[i] = p->k_stride[i]; g.vs[i] = p->v_stride[i]; g.os[i] = p->o_stride[i]; }
     g.buckets = p->num_buckets;
     g.q_tiles = (int)ceil_div(p->sq, kQueryTile);
-    if ((int64_t)g.q_tiles * g.batch * g.heads > 0x7fffffff) return set_error(BH_EINVAL, "%s: too many query tiles", fn);
+    if ((int64_t)g.q_tiles * g.batch * g.heads > kMostGroups || ceil_div(p->sk, 128) * g.batch * g.heads > kMostGroups ||
+        ceil_div(g.buckets, 16) * g.heads > kMostGroups)
+        return set_error(BH_EINVAL, "%s: too many rows", fn);
     return BH_OK;
 }
 
@@ -1057,42 +1085,71 @@ static int launch_lds(K kernel, bool& raised, dim3 grid, int bytes, const char* 
 // planes of several operands in one launch
 struct Planes {
     SplitJobs jobs = {};
-    int n = 0, total = 0;
+    int n = 0;
+    int64_t total = 0;
     void add(const float* src, const int64_t (&s)[3], int heads, int batch, int64_t rows, const int32_t* len, int blocks, bool vec, const char* row,
              const char* col) {
         SplitJob& j = jobs.j[n];
         j.src = src; j.heads = heads; j.rows = rows; j.len = len; j.blocks = blocks; j.vec = vec;
         j.row = const_cast<char*>(row); j.col = const_cast<char*>(col);
         for (int i = 0; i < 3; i++) j.s[i] = s[i];
-        total += batch * heads * blocks;
-        for (int i = ++n; i <= kMaxJobs; i++) jobs.first[i] = total;
+        total += (int64_t)batch * heads * blocks;
+        for (int i = ++n; i <= kMaxJobs; i++) jobs.first[i] = (int)(total < kMostGroups ? total : kMostGroups);
     }
     SplitJob& last() { return jobs.j[n - 1]; }
     template <int DP> int launch(int d) {
+        if (total > kMostGroups) return set_error(BH_EINVAL, "bh_relbias_attention: too many rows");
         jobs.d = d;
         hipLaunchKernelGGL(relattn_split_kernel<DP>, dim3((unsigned)total), dim3(256), 0, stream(), jobs);
         return BH_LAUNCH_CHECK("bh_relbias_attention: split");
     }
 };
 
-static int g_force_rows = -1;
+static int g_force_rows = -1, g_force_splits = 0;
+
+// Parts into which the walk of `wgs` workgroups is cut, `each` of which share one of the 256 compute units: the longest walk has
+// `longest` steps, `mean` is the average.  Where all are alike the rounds of workgroups count, else (longest first) the longest
+// walk or all the work spread evenly.  A part's start counts as `start` steps, joining as `join` a part.
+// Backward, us, head size 64, causal, whole / in parts as chosen: 64 queries of 8 heads over 4096 keys 303 / 68, 16 heads of 512
+// 122 / 64, of 2048 365 / 284; 128 heads of 1024 491 in one part, 578 in two.  Forward: 64 sequences of one query over 8001 keys
+// 187 / 52, 16 heads of 2048 106 / 83; 64 heads of 256 23 in one part, 39 in two.
+static int parts_for(int64_t wgs, int64_t longest, double mean, int each, int start, double join, int most) {
+    if (g_force_splits > 0) return (int)(g_force_splits < longest ? g_force_splits : longest > 0 ? longest : 1);
+    const int64_t slots = 256 * each;
+    int best = 1;
+    double least = INFINITY;
+    for (int s = 1; s <= most && s <= longest; s++) {
+        const double walk = (double)(ceil_div(longest, s) + start), all = (double)(wgs * s) / (double)slots * (mean / s + start);
+        const double cost = (mean >= (double)(longest - 1) ? (double)ceil_div(wgs * s, slots) * walk : walk > all ? walk : all) + (s > 1 ? join * (s + 1) : 0.0);
+        if (cost < 0.97 * least) { least = cost; best = s; }
+    }
+    return best;
+}
+// the pairs of query and key that a causal mask leaves
+static double seen_pairs(const RelArgs& g) {
+    if (!g.causal) return (double)g.sq * (double)g.sk;
+    // query i sees min(max(i + 1 + offset, 0), sk) keys: none below lo, all from hi on
+    const int64_t lo = -g.offset < 0 ? 0 : -g.offset < g.sq ? -g.offset : g.sq, full = g.sk - 1 - g.offset;
+    const int64_t hi = full < lo ? lo : full < g.sq ? full : g.sq;
+    return ((double)(lo + 1 + g.offset) + (double)(hi + g.offset)) * 0.5 * (double)(hi - lo) + (double)(g.sq - hi) * (double)g.sk;
+}
 
 template <int DP>
 static int run_forward(RelArgs& g) {
     static bool raised = false;
     const int64_t rows = (int64_t)g.batch * g.heads * g.sq;
     const int64_t head_rows = (int64_t)g.group * g.sq, row_tiles = ceil_div(head_rows, 32);
-    const bool by_rows = g_force_rows >= 0 ? g_force_rows == 1 && head_rows < (1 << 24) : row_tiles <= 2;
+    // The kernel for few rows reads (and splits) the keys once per 32 rows, the tiles need planes made first (us, rows / tiles,
+    // head size 64): 64 rows of 128 heads over 4096 keys 112 / 218, 128 rows 193 / 229, of 8 heads 28 / 33, 64 over 128 keys of
+    // 96 heads 12 / 20; 128 over 512 keys of 256 heads 64 / 64, over 128 keys of 384 heads 44 / 33, 192 over 192 33 / 24.
+    const bool by_rows = g_force_rows >= 0 ? g_force_rows == 1 && head_rows < (1 << 24) : row_tiles <= 2 || (row_tiles <= 4 && g.sk >= 2 * head_rows);
     const int64_t wgs = by_rows ? row_tiles * g.batch * g.kv_heads : (int64_t)g.q_tiles * g.batch * g.heads;
-    if (wgs > 0x7fffffff) return set_error(BH_EINVAL, "bh_relbias_attention_forward: too many rows");
-    // the keys are cut where the workgroups are few: to about three per compute unit, a cut being 64 keys a wavefront at least
+    if (wgs > kMostGroups) return set_error(BH_EINVAL, "bh_relbias_attention_forward: too many rows");
     const int64_t unit = by_rows ? 32 * kRowWaves : 64, tiles = ceil_div(g.sk, unit);
-    int64_t splits = 1;
-    if (wgs < 512 && tiles >= 4) {
-        splits = ceil_div(768, wgs);
-        if (splits > tiles / 2) splits = tiles / 2;
-        if (splits > 64) splits = 64;
-    }
+    const int each = !by_rows ? 2 : DP <= 32 ? 4 : DP <= 96 ? 2 : 1;
+    // a step takes about 2.5 us, in which 10 MB of parts are written and read again
+    const double join = 0.05 + (double)rows * g.d * 8e-7;
+    const int splits = parts_for(wgs, tiles, seen_pairs(g) / ((double)unit * (double)g.sq), each, 2, join, 64);
     g.keys_per_split = ceil_div(tiles > 0 ? tiles : 1, splits) * unit;
     g.splits = (int)ceil_div(g.sk > 0 ? g.sk : 1, g.keys_per_split);
     Scratch part, planes;
@@ -1130,57 +1187,58 @@ static int run_forward(RelArgs& g) {
 template <int DP>
 static int run_backward(RelArgs& g, float* dtable, int accumulate) {
     static bool raised_q = false, raised_k = false;
-    const int64_t rows = (int64_t)g.batch * g.heads * g.sq, wgs = (int64_t)g.q_tiles * g.batch * g.heads;
-    Scratch delta, table, planes;
-    if (!delta.get(sizeof(float) * (size_t)rows) || !table.get(sizeof(double) * (size_t)wgs * (size_t)g.buckets)) return BH_ENOMEM;
+    const int64_t nbh = (int64_t)g.batch * g.heads, rows = nbh * g.sq, wgs = (int64_t)g.q_tiles * nbh;
+    const int k_tiles = (int)ceil_div(g.sk, 128), each = DP <= 64 ? 2 : 1;
+    // dQ walks over a tile's keys, dK and dV over the queries that see one
+    const int64_t k_steps = ceil_div(g.sk, 32), q_steps = ceil_div(g.sq, 32);
+    const double pairs = seen_pairs(g);
+    g.keys_per_split = ceil_div(k_steps > 0 ? k_steps : 1, parts_for(wgs, k_steps, pairs / (32.0 * g.sq), each, 5, 0, 32)) * 32;
+    g.splits = g.sk > 0 ? (int)ceil_div(g.sk, g.keys_per_split) : 1;
+    g.queries_per_split = (int)ceil_div(q_steps, parts_for(k_tiles * nbh, q_steps, g.sk > 0 ? pairs / (32.0 * g.sk) : 0.0, each, 5, 0, 32)) * 32;
+    g.q_splits = (int)ceil_div(g.sq, g.queries_per_split);
+    Scratch delta, table, planes, part_q, part_kv;
+    if (!delta.get(sizeof(float) * (size_t)rows) || !table.get(sizeof(double) * (size_t)g.splits * (size_t)wgs * (size_t)g.buckets)) return BH_ENOMEM;
     g.delta = (float*)delta.p;
     g.part_table = (double*)table.p;
-    int rc;
-    {
-        g.k_blocks = (int)ceil_div(g.sk, 64) * 2;
-        g.q_blocks = (int)ceil_div(g.sq, 32);
-        const size_t kb = (size_t)g.batch * g.kv_heads * g.k_blocks * Block<DP>::BYTES, qb = (size_t)g.batch * g.heads * g.q_blocks * Block<DP>::BYTES;
-        if (!planes.get(3 * kb + 4 * qb)) return BH_ENOMEM;   // no keys: the planes of the queries alone are made, for the dots
-        g.k_row = (const char*)planes.p; g.k_col = g.k_row + kb; g.v_row = g.k_col + kb;
-        g.q_row = g.v_row + kb; g.q_col = g.q_row + qb; g.g_row = g.q_col + qb; g.g_col = g.g_row + qb;
-        Planes p;
-        if (g.sk > 0) {
-            p.add(g.k, g.ks, g.kv_heads, g.batch, g.sk, g.kv_len, g.k_blocks, g.vec_k, g.k_row, g.k_col);
-            p.add(g.v, g.vs, g.kv_heads, g.batch, g.sk, g.kv_len, g.k_blocks, g.vec_v, g.v_row, nullptr);
-        }
-        p.add(g.q, g.qs, g.heads, g.batch, g.sq, nullptr, g.q_blocks, g.vec_q, g.q_row, g.q_col);
-        p.add(g.d_out, g.os, g.heads, g.batch, g.sq, nullptr, g.q_blocks, g.vec_o, g.g_row, g.g_col);
-        p.last().with = g.out_in;
-        p.last().dots = g.delta;
-        rc = p.launch<DP>(g.d);
-        if (rc) return rc;
+    if (g.splits > 1) {
+        if (!part_q.get(sizeof(float) * (size_t)g.splits * (size_t)rows * g.d)) return BH_ENOMEM;
+        g.part_q = (float*)part_q.p;
     }
-    rc = launch_lds(&relattn_dq_kernel<DP>, raised_q, dim3((unsigned)wgs), QueryLds<DP>::BYTES, "bh_relbias_attention_backward: dq", g);
+    if (g.sk > 0 && (g.group > 1 || g.q_splits > 1)) {
+        const size_t size = (size_t)g.q_splits * nbh * (size_t)g.sk * g.d;
+        if (!part_kv.get(2 * sizeof(float) * size)) return BH_ENOMEM;
+        g.part_k = (float*)part_kv.p;
+        g.part_v = g.part_k + size;
+    }
+    g.k_blocks = (int)ceil_div(g.sk, 64) * 2;
+    g.q_blocks = (int)ceil_div(g.sq, 32);
+    const size_t kb = (size_t)g.batch * g.kv_heads * g.k_blocks * Block<DP>::BYTES, qb = (size_t)nbh * g.q_blocks * Block<DP>::BYTES;
+    if (!planes.get(3 * kb + 4 * qb)) return BH_ENOMEM;       // no keys: the planes of the queries alone are made, for the dots
+    g.k_row = (const char*)planes.p; g.k_col = g.k_row + kb; g.v_row = g.k_col + kb;
+    g.q_row = g.v_row + kb; g.q_col = g.q_row + qb; g.g_row = g.q_col + qb; g.g_col = g.g_row + qb;
+    Planes p;
+    if (g.sk > 0) {
+        p.add(g.k, g.ks, g.kv_heads, g.batch, g.sk, g.kv_len, g.k_blocks, g.vec_k, g.k_row, g.k_col);
+        p.add(g.v, g.vs, g.kv_heads, g.batch, g.sk, g.kv_len, g.k_blocks, g.vec_v, g.v_row, nullptr);
+    }
+    p.add(g.q, g.qs, g.heads, g.batch, g.sq, nullptr, g.q_blocks, g.vec_q, g.q_row, g.q_col);
+    p.add(g.d_out, g.os, g.heads, g.batch, g.sq, nullptr, g.q_blocks, g.vec_o, g.g_row, g.g_col);
+    p.last().with = g.out_in;
+    p.last().dots = g.delta;
+    int rc = p.launch<DP>(g.d);
     if (rc) return rc;
-    hipLaunchKernelGGL(relattn_table_kernel, dim3((unsigned)ceil_div(g.buckets, 16), (unsigned)g.heads), dim3(256), 0, stream(), g, dtable, accumulate);
-    rc = BH_LAUNCH_CHECK("bh_relbias_attention_backward: table");
-    if (rc || g.sk == 0) return rc;
-    if (!raised_k) {
-        rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(&relattn_dkv_kernel<DP>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                           KeyLds<DP>::BYTES), "bh_relbias_attention_backward: LDS size");
+    rc = launch_lds(&relattn_dq_kernel<DP>, raised_q, dim3((unsigned)wgs, (unsigned)g.splits), QueryLds<DP>::BYTES, "bh_relbias_attention_backward: dq", g);
+    if (rc) return rc;
+    if (g.sk > 0) {
+        rc = launch_lds(&relattn_dkv_kernel<DP>, raised_k, dim3((unsigned)(k_tiles * nbh), (unsigned)g.q_splits), KeyLds<DP>::BYTES,
+                        "bh_relbias_attention_backward: dk, dv", g);
         if (rc) return rc;
-        raised_k = true;
     }
-    Scratch heads;
-    if (g.group > 1) {
-        const size_t each = (size_t)g.batch * g.heads * (size_t)g.sk * g.d;
-        if (!heads.get(2 * sizeof(float) * each)) return BH_ENOMEM;
-        g.part_k = (float*)heads.p;
-        g.part_v = g.part_k + each;
-    }
-    const int k_tiles = (int)ceil_div(g.sk, 128);
-    hipLaunchKernelGGL(relattn_dkv_kernel<DP>, dim3((unsigned)((int64_t)k_tiles * g.batch * g.heads)), dim3(kThreads), KeyLds<DP>::BYTES, stream(),
-                       g, k_tiles);
-    rc = BH_LAUNCH_CHECK("bh_relbias_attention_backward: dk, dv");
-    if (rc || g.group == 1) return rc;
-    const int64_t blocks = ceil_div((int64_t)g.batch * g.kv_heads * g.sk * g.d, 256);
-    hipLaunchKernelGGL(relattn_heads_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream(), g);
-    return BH_LAUNCH_CHECK("bh_relbias_attention_backward: heads");
+    const auto blocks = [](int64_t n) { const int64_t b = ceil_div(n, 256); return (int)(b < 4096 ? b : 4096); };
+    const Fold f = {(int)ceil_div(g.buckets, 16) * g.heads, g.splits > 1 ? blocks(rows * g.d) : 0,
+                    g.part_k ? blocks((int64_t)g.batch * g.kv_heads * g.sk * g.d) : 0, dtable, accumulate};
+    hipLaunchKernelGGL(relattn_fold_kernel, dim3((unsigned)(f.table_blocks + f.q_blocks + f.k_blocks)), dim3(256), 0, stream(), g, f);
+    return BH_LAUNCH_CHECK("bh_relbias_attention_backward: fold");
 }
 
 }  // namespace bh
@@ -1206,6 +1264,12 @@ int bh_relative_position_bucket(int64_t relative, int num_buckets, int max_dista
 int bh_relbias_attention_force_rows(int mode) {
     BH_CHECK_ARG(mode >= -1 && mode <= 1, "-1, 0 or 1");
     g_force_rows = mode;
+    return BH_OK;
+}
+
+int bh_relbias_attention_force_splits(int splits) {
+    BH_CHECK_ARG(splits >= 0 && splits <= 64, "0 to 64");
+    g_force_splits = splits;
     return BH_OK;
 }
 

@@ -93,7 +93,7 @@ _SIGS = {
     "bh_sdpa_forward_cached": (I, [P, P, P, F, I, P, P, P, L, L, L]),
     "bh_sdpa_backward_cached": (I, [P, P, P, P, P, P, P, F, I, P, P, P, L, L, L]),
     "bh_relative_position_bucket": (I, [L, I, I, I]),
-    "bh_relbias_attention_force_rows": (I, [I]),
+    "bh_relbias_attention_force_rows": (I, [I]), "bh_relbias_attention_force_splits": (I, [I]),
     "bh_relbias_attention_forward": (I, [C.POINTER(RelbiasAttention)] + [P] * 7),
     "bh_relbias_attention_backward": (I, [C.POINTER(RelbiasAttention)] + [P] * 12 + [I]),
     "bh_adam_update": (I, [P, P, P, P, L, F, F, F, F, L]),

@@ -404,6 +404,9 @@ int bh_gemm_no_tables(int off);
 int bh_sdpa_force_general(int on);
 /* bh_relbias_attention_force_rows: 1 = the forward pass's kernel for few query rows, 0 = its tiles, -1 = by shape (default) */
 int bh_relbias_attention_force_rows(int mode);
+/* bh_relbias_attention_force_splits: parts into which the keys (forward, dq) and the queries (dk, dv) are cut; 0 = by shape
+ * (default) */
+int bh_relbias_attention_force_splits(int splits);
 /* bh_gemm_epilogue_force: variant 0 = 256x256, 1 = 128x128 tiles through LDS, 2 = 32x32, 3 = 64x64, 4 = 32x32 with sixteen
  * wavefronts (small problems), -1 = by shape (default); splits > 0: cut the contraction this many ways, 0 = by shape */
 int bh_gemm_epilogue_force(int variant, int splits);

@@ -567,6 +567,19 @@ def test_attention_training_of_a_longer_sequence(hip, rng):
     check_attention(hip, attention_case(rng, 1, 1, 1, 500, 700, 128, 64), both=True, causal=False, distance=1024)
 
 
+@pytest.mark.parametrize("splits", [1, 2, 3, 64])
+@pytest.mark.parametrize("d", [24, 64, 96, 128])
+def test_attention_backward_in_parts(hip, rng, splits, d):
+    """The keys of dq and the queries of dk and dv cut into parts, some of them past a causal mask's or a sequence's end."""
+    hip.check(hip.bh_relbias_attention_force_splits(splits))
+    try:
+        check_attention(hip, attention_case(rng, 2, 4, 2, 150, 230, d, 16), lens=[230, 41])
+        check_attention(hip, attention_case(rng, 2, 2, 2, 40, 300, d, 16), lens=[0, 300], causal=False, both=True, order=(0, 2, 1), pad=3)
+        check_attention(hip, attention_case(rng, 1, 2, 1, 300, 20, d, 16), offset=-100)
+    finally:
+        hip.check(hip.bh_relbias_attention_force_splits(0))
+
+
 def test_attention_large_scores(hip, rng):
     q, k, v, table, d_out = attention_case(rng, 1, 2, 2, 70, 100, 64, 16)
     check_attention(hip, (q * 6, k * 6, v, table * 20, d_out), scale=0.3)
