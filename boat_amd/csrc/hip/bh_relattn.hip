@@ -579,43 +579,83 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 96 ? 2 : 1) void relattn_rows
     if (wave == 0 && 32 * rt + (lane & 31) < rows) store_forward<DP>(g, o, top, sum, bt * g.heads + h, qi, blockIdx.y, lane);
 }
 
-// the splits' parts of a row: one wavefront per row, a lane per split (at most 64) for the weights
+// the splits' parts of a row: 16 lanes a row, which hold the weights of at most 64 splits
 __global__ __launch_bounds__(256) void relattn_join_kernel(RelArgs g) {
-    const int64_t rows = (int64_t)g.batch * g.heads * g.sq;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (row >= rows) return;
-    float m = -INFINITY, l = 0.f;
-    if (lane < g.splits) {
-        const f32x2 ml = *reinterpret_cast<const f32x2*>(g.part_ml + 2 * (lane * rows + row));
-        m = ml[0];
-        l = ml[1];
+    const int64_t rows = (int64_t)g.batch * g.heads * g.sq, mine = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int64_t row = min(mine, rows - 1);
+    const int lane = threadIdx.x & 15;
+    float m[4], l[4], top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+        if (lane + 16 * i < g.splits) {
+            const f32x2 ml = *reinterpret_cast<const f32x2*>(g.part_ml + 2 * ((lane + 16 * i) * rows + row));
+            m[i] = ml[0];
+            l[i] = ml[1];
+        }
+        top = fmaxf(top, m[i]);
     }
-    const float top = wave_max(m), base = top == -INFINITY ? 0.f : top;
-    const float w = __builtin_amdgcn_exp2f(m - base);                         // 0 for a lane without a split
-    const float sum = wave_sum(l * w);
-    const int64_t bh = row / g.sq, qi = row % g.sq;
-    float* dst = g.out + bh / g.heads * g.os[0] + bh % g.heads * g.os[1] + qi * g.os[2];
+#pragma unroll
+    for (int x = 1; x < 16; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
+    const float base = top == -INFINITY ? 0.f : top;
+    float w[4], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        w[i] = __builtin_amdgcn_exp2f(m[i] - base);                           // 0 where there is no split
+        sum += l[i] * w[i];
+    }
+#pragma unroll
+    for (int x = 1; x < 16; x *= 2) sum += __shfl_xor(sum, x, 64);
+    const int64_t bh = row / g.sq, qi = row - bh * g.sq, bt = bh / g.heads, h = bh - bt * g.heads;
+    float* dst = g.out + bt * g.os[0] + h * g.os[1] + qi * g.os[2];
     const float f = top == -INFINITY ? 0.f : 1.f / sum;
-    for (int c = lane; c < (g.d + 63) / 64 * 64; c += 64) {
-        const float* p = g.part_o + row * g.d + min(c, g.d - 1);
-        float a = 0.f;
-        for (int s0 = 0; s0 < g.splits; s0 += 8) {                            // eight loads at a time; past the last split weight 0
-            float x[8];
+    const bool vec = g.d % 4 == 0;
+    for (int c0 = 0; c0 < g.d; c0 += 64) {
+        const int c = c0 + 4 * lane, n = min(4, g.d - c), at = min(c, g.d - 1) & (vec ? ~3 : ~0);
+        const float* p = g.part_o + row * g.d + at;
+        f32x4 a = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = 0; s0 < g.splits; s0 += 4) {                            // four loads at a time; past the last split weight 0
+            f32x4 x[4];
 #pragma unroll
-            for (int s = 0; s < 8; s++) x[s] = p[min(s0 + s, g.splits - 1) * rows * g.d];
+            for (int s = 0; s < 4; s++) {
+                const float* from = p + min(s0 + s, g.splits - 1) * rows * g.d;
+                if (vec) x[s] = *reinterpret_cast<const f32x4*>(from);
+                else
 #pragma unroll
-            for (int s = 0; s < 8; s++) {
-                const float y = __shfl(w, s0 + s, 64);
-                a += y == 0.f ? 0.f : y * x[s];
+                    for (int j = 0; j < 4; j++) x[s][j] = from[max(0, min(j, n - 1))];
+            }
+            const int i = s0 >> 4;
+            const float ws = i == 0 ? w[0] : i == 1 ? w[1] : i == 2 ? w[2] : w[3];
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const float y = __shfl(ws, (threadIdx.x & 48) + ((s0 + s) & 15), 64);
+#pragma unroll
+                for (int j = 0; j < 4; j++) a[j] += y == 0.f ? 0.f : y * x[s][j];
             }
         }
-        if (c < g.d) dst[c] = a * f;
+        if (mine < rows && n > 0) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) a[j] *= f;
+            if (g.vec_o) *reinterpret_cast<f32x4*>(dst + c) = a;
+            else
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (j < n) dst[c + j] = a[j];
+        }
     }
-    if (lane == 0) g.lse[row] = top == -INFINITY ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (mine < rows && lane == 0) g.lse[row] = top == -INFINITY ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------------------------------- backward
+// The kernel's arguments read anew, where a walk is over: kept from its start on they would hold scalar registers through it
+// (they are the kernel's first parameter).
+using Arguments = const __attribute__((address_space(4))) RelArgs;
+__device__ __forceinline__ Arguments* arguments_again() {
+    Arguments* a = (Arguments*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    return a;
+}
 // log2 e * lse; rows that see nothing get a number (their scores are all masked)
 __device__ __forceinline__ float lse_log2(float lse) { return lse == -INFINITY ? 0.f : lse * kLog2e; }
 
@@ -629,7 +669,7 @@ template <int DP> struct QueryLds {
 
 // dQ and the table's gradient: a workgroup owns 128 queries of a head and walks over the keys
 template <int DP>
-__global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(RelArgs g) {
+__device__ __forceinline__ void query_tile(const RelArgs& g, int id, int part) {
     using L = QueryLds<DP>;
     constexpr int KEYS = 32, ND = DP / 32, KD = DP / 16, KB = Block<DP>::BYTES / 1024;
     extern __shared__ __align__(16) char smem[];
@@ -637,7 +677,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
     double* sums = reinterpret_cast<double*>(smem + L::SUMS) + kMaxBuckets * wave;
     float* block = reinterpret_cast<float*>(smem + L::BLOCK) + 32 * 33 * wave;
     int bh, tile;
-    head_and_tile(blockIdx.x, g.batch * g.heads, g.q_tiles, g.causal, bh, tile);
+    head_and_tile(id, g.batch * g.heads, g.q_tiles, g.causal, bh, tile);
     const int bt = bh / g.heads, h = bh % g.heads, hk = h / g.group;
     const float* q = g.q + bt * g.qs[0] + h * g.qs[1];
     const float* dout = g.d_out + bt * g.os[0] + h * g.os[1];
@@ -650,7 +690,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
     const int len = g.kv_len ? min(max(g.kv_len[bt], 0), (int)g.sk) : (int)g.sk;
     int ke = len;
     if (g.causal) ke = (int)min((int64_t)ke, max((int64_t)0, min((int64_t)q0 + kQueryTile, g.sq) + g.offset));
-    const int kb = (int)(blockIdx.y * g.keys_per_split);
+    const int kb = (int)(part * g.keys_per_split);
     ke = (int)min((int64_t)ke, kb + g.keys_per_split);
     const int rel_q = (int)(qw + g.offset);
     const auto fetch_rows = [&](int k0) {
@@ -763,26 +803,27 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dq_kernel(
     }
     __syncthreads();
     const double* all = reinterpret_cast<const double*>(smem + L::SUMS);
-    const int64_t split_bh = (int64_t)blockIdx.y * g.batch * g.heads;
+    const int64_t split_bh = (int64_t)part * g.batch * g.heads;
     for (int i = tid; i < g.buckets; i += kThreads)
         g.part_table[((split_bh + bh) * g.q_tiles + tile) * g.buckets + i] =
             (all[i] + all[kMaxBuckets + i]) + (all[2 * kMaxBuckets + i] + all[3 * kMaxBuckets + i]);
     if (!live) return;
-    const bool part = g.splits > 1, vec = part ? g.d % 4 == 0 : g.vec_q;
-    float* dst = part ? g.part_q + ((split_bh + bh) * g.sq + qi) * g.d : g.dq + bt * g.qs[0] + h * g.qs[1] + qi * g.qs[2];
+    Arguments& e = *arguments_again();
+    const bool parts = e.splits > 1, vec = parts ? e.d % 4 == 0 : e.vec_q;
+    float* dst = parts ? e.part_q + ((split_bh + bh) * e.sq + qi) * e.d : e.dq + bt * e.qs[0] + h * e.qs[1] + qi * e.qs[2];
 #pragma unroll
     for (int b = 0; b < DP / 32; b++)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int cd = 32 * b + acc_row(e, lane);
+        for (int r = 0; r < 16; r += 4) {
+            const int cd = 32 * b + acc_row(r, lane);
             f32x4 y;
 #pragma unroll
-            for (int j = 0; j < 4; j++) y[j] = dq[b][e + j] * g.scale;
-            if (vec && cd + 4 <= g.d) *reinterpret_cast<f32x4*>(dst + cd) = y;
+            for (int j = 0; j < 4; j++) y[j] = dq[b][r + j] * e.scale;
+            if (vec && cd + 4 <= e.d) *reinterpret_cast<f32x4*>(dst + cd) = y;
             else
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    if (cd + j < g.d) dst[cd + j] = y[j];
+                    if (cd + j < e.d) dst[cd + j] = y[j];
         }
 }
 
@@ -797,14 +838,14 @@ template <int DP> struct KeyLds {
 // dK and dV of one query head: a workgroup owns 128 keys and walks over the queries.  Heads that share a key head leave their
 // parts in work memory (one long chain of sums over all of them would round more, and fill fewer compute units)
 template <int DP>
-__global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel(RelArgs g) {
+__device__ __forceinline__ void key_tile(const RelArgs& g, int id, int part) {
     using L = KeyLds<DP>;
     constexpr int ROWS = 32, ND = DP / 32, KD = DP / 16, KB = Block<DP>::BYTES / 1024;
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int bh, tile;
     const int k_tiles = (int)((g.sk + 127) / 128);
-    head_and_tile(blockIdx.x, g.batch * g.heads, k_tiles, g.causal, bh, tile);
+    head_and_tile(id, g.batch * g.heads, k_tiles, g.causal, bh, tile);
     tile = k_tiles - 1 - tile;                                                // the first keys are seen by the most queries
     const int bt = bh / g.heads, h = bh % g.heads, hk = h / g.group;
     const float* k = g.k + bt * g.ks[0] + hk * g.ks[1];
@@ -827,8 +868,8 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
     const float c = g.scale * kLog2e;
     int qb = 0;                                                               // causal: the first query that sees a key of the workgroup
     if (g.causal) qb = (int)(min((int64_t)sq, max((int64_t)0, (int64_t)tile * 128 - g.offset)) / ROWS * ROWS);
-    const int qe = min(sq, (int)(blockIdx.y + 1) * g.queries_per_split);
-    qb = max(qb, (int)blockIdx.y * g.queries_per_split);
+    const int qe = min(sq, (part + 1) * g.queries_per_split);
+    qb = max(qb, part * g.queries_per_split);
     if (tile * 128 >= len) qb = sq;                                           // only padding here
     // One turn of a loop that the compiler cannot see to be one: it then keeps the fragments' making apart from the steps.
     // Run together they need 47 registers more than there are at head size 128.
@@ -914,40 +955,87 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_dkv_kernel
             wait_copies();
         }
     }
-    if (ki >= g.sk) return;
-    const bool part = g.part_k;
-    const int64_t at = (((int64_t)blockIdx.y * g.batch * g.heads + bh) * g.sk + ki) * g.d;
-    float* pk = part ? g.part_k + at : g.dk + bt * g.ks[0] + hk * g.ks[1] + ki * g.ks[2];
-    float* pv = part ? g.part_v + at : g.dv + bt * g.vs[0] + hk * g.vs[1] + ki * g.vs[2];
-    const bool vec_k = part ? g.d % 4 == 0 : g.vec_k, vec_v = part ? g.d % 4 == 0 : g.vec_v;
+    Arguments& e = *arguments_again();
+    int again = threadIdx.x;
+    asm volatile("" : "+v"(again));
+    const int kj = tile * 128 + again / 64 * 32 + (again & 31);
+    if (kj >= e.sk) return;
+    const bool parts = e.part_k;
+    const int64_t at = (((int64_t)part * e.batch * e.heads + bh) * e.sk + kj) * e.d;
+    float* pk = parts ? e.part_k + at : e.dk + bt * e.ks[0] + hk * e.ks[1] + kj * e.ks[2];
+    float* pv = parts ? e.part_v + at : e.dv + bt * e.vs[0] + hk * e.vs[1] + kj * e.vs[2];
+    const bool vec_k = parts ? e.d % 4 == 0 : e.vec_k, vec_v = parts ? e.d % 4 == 0 : e.vec_v;
 #pragma unroll
     for (int b = 0; b < ND; b++)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int cd = 32 * b + acc_row(e, lane);
+        for (int r = 0; r < 16; r += 4) {
+            const int cd = 32 * b + acc_row(r, again & 63);
             f32x4 x, y;
 #pragma unroll
-            for (int j = 0; j < 4; j++) { x[j] = dk[b][e + j] * g.scale; y[j] = dv[b][e + j]; }
-            if (vec_k && cd + 4 <= g.d) *reinterpret_cast<f32x4*>(pk + cd) = x;
+            for (int j = 0; j < 4; j++) { x[j] = dk[b][r + j] * e.scale; y[j] = dv[b][r + j]; }
+            if (vec_k && cd + 4 <= e.d) *reinterpret_cast<f32x4*>(pk + cd) = x;
             else
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    if (cd + j < g.d) pk[cd + j] = x[j];
-            if (vec_v && cd + 4 <= g.d) *reinterpret_cast<f32x4*>(pv + cd) = y;
+                    if (cd + j < e.d) pk[cd + j] = x[j];
+            if (vec_v && cd + 4 <= e.d) *reinterpret_cast<f32x4*>(pv + cd) = y;
             else
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    if (cd + j < g.d) pv[cd + j] = y[j];
+                    if (cd + j < e.d) pv[cd + j] = y[j];
             __builtin_amdgcn_sched_barrier(0);
         }
 }
 
+// Both walks in one launch: the key tiles, which take longer, first, and the query tiles fill up behind them (one launch after the
+// other, us: 128 heads of 1024, causal, 482 against 459; 32 heads of 1024 at head size 128 379 against 261)
+template <int DP>
+__global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_backward_kernel(RelArgs g, int key_groups, int query_groups) {
+    const int all_keys = key_groups * g.q_splits, id = blockIdx.x;
+    const bool keys = id < all_keys;
+    const int at = keys ? id : id - all_keys, groups = keys ? key_groups : query_groups;
+    const int part = __builtin_amdgcn_readfirstlane(at / groups), tile = __builtin_amdgcn_readfirstlane(at - part * groups);
+    if (keys) key_tile<DP>(g, tile, part);
+    else query_tile<DP>(g, tile, part);
+}
+
+// n floats (at most 4) of parts that lie `step` apart, `count` of them, added up in order
+__device__ __forceinline__ f32x4 sum_of(const float* p, int64_t step, int count, int n, bool vec, f32x4 t) {
+    for (int i = 0; i < count; i += 4) {
+        f32x4 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const float* at = p + min(i + u, count - 1) * step;
+            if (vec) x[u] = *reinterpret_cast<const f32x4*>(at);
+            else
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[u][j] = at[min(j, n - 1)];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) t[j] += i + u < count ? x[u][j] : 0.f;
+    }
+    return t;
+}
+__device__ __forceinline__ void put(float* dst, f32x4 t, int n, bool vec) {
+    if (vec) *reinterpret_cast<f32x4*>(dst) = t;
+    else
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (j < n) dst[j] = t[j];
+}
+
 // What is left in parts, added up in order: the first workgroups make dT (16 buckets of a head each, over splits, batch and
-// tiles), the next ones dQ where the keys were split, the last ones dK and dV where the queries were or heads share a key head.
+// tiles), the next ones dQ where the keys were split, the last ones dK and dV where the queries were or heads share a key head;
+// 16 or 32 lanes a row, four floats a lane.
 struct Fold { int table_blocks, q_blocks, k_blocks; float* dtable; int accumulate; };
 __global__ __launch_bounds__(256) void relattn_fold_kernel(RelArgs g, Fold f) {
     __shared__ double red[256];
-    const int id = blockIdx.x;
+    const int id = blockIdx.x, lanes = g.d <= 64 ? 16 : 32, c = threadIdx.x % lanes * 4, per_block = 256 / lanes;
+    const int n = min(4, g.d - c), slot = threadIdx.x / lanes;
+    const bool vec = g.d % 4 == 0;
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     if (id < f.table_blocks) {
         const int h = id % g.heads, b = id / g.heads * 16 + (threadIdx.x & 15), first = threadIdx.x >> 4;
         const int64_t total = (int64_t)g.splits * g.batch * g.q_tiles;
@@ -965,24 +1053,26 @@ __global__ __launch_bounds__(256) void relattn_fold_kernel(RelArgs g, Fold f) {
             float* dst = f.dtable + (int64_t)b * g.heads + h;
             *dst = f.accumulate ? *dst + (float)t : (float)t;
         }
+    } else if (n <= 0) {
+        return;
     } else if (id < f.table_blocks + f.q_blocks) {
-        const int64_t per = g.sq * g.d, total = (int64_t)g.batch * g.heads * per;
-        for (int64_t i = (int64_t)(id - f.table_blocks) * 256 + threadIdx.x; i < total; i += (int64_t)f.q_blocks * 256) {
-            const int64_t bh = i / per, at = i - bh * per, row = at / g.d, c = at - row * g.d, bt = bh / g.heads, h = bh - bt * g.heads;
-            float x = g.part_q[i];
-            for (int p = 1; p < g.splits; p++) x += g.part_q[i + p * total];
-            g.dq[bt * g.qs[0] + h * g.qs[1] + row * g.qs[2] + c] = x;
+        const int64_t rows = (int64_t)g.batch * g.heads * g.sq;
+        for (int64_t r = (int64_t)(id - f.table_blocks) * per_block + slot; r < rows; r += (int64_t)f.q_blocks * per_block) {
+            const int64_t bh = r / g.sq, row = r - bh * g.sq, bt = bh / g.heads, h = bh - bt * g.heads;
+            put(g.dq + bt * g.qs[0] + h * g.qs[1] + row * g.qs[2] + c, sum_of(g.part_q + r * g.d + c, rows * g.d, g.splits, n, vec, zero), n, vec && g.vec_q);
         }
     } else {
-        const int64_t per = g.sk * g.d, total = (int64_t)g.batch * g.kv_heads * per, all = (int64_t)g.batch * g.heads * per;
-        for (int64_t i = (int64_t)(id - f.table_blocks - f.q_blocks) * 256 + threadIdx.x; i < total; i += (int64_t)f.k_blocks * 256) {
-            const int64_t bk = i / per, at = i - bk * per, row = at / g.d, c = at - row * g.d, bt = bk / g.kv_heads, hk = bk - bt * g.kv_heads;
-            const int64_t first = (bt * g.heads + hk * g.group) * per + at;
-            float x = 0.f, y = 0.f;
-            for (int p = 0; p < g.q_splits; p++)
-                for (int h = 0; h < g.group; h++) { x += g.part_k[first + h * per + p * all]; y += g.part_v[first + h * per + p * all]; }
-            g.dk[bt * g.ks[0] + hk * g.ks[1] + row * g.ks[2] + c] = x;
-            g.dv[bt * g.vs[0] + hk * g.vs[1] + row * g.vs[2] + c] = y;
+        const int64_t rows = (int64_t)g.batch * g.kv_heads * g.sk, per = g.sk * g.d, all = (int64_t)g.batch * g.heads * per;
+        for (int64_t r = (int64_t)(id - f.table_blocks - f.q_blocks) * per_block + slot; r < rows; r += (int64_t)f.k_blocks * per_block) {
+            const int64_t bk = r / g.sk, row = r - bk * g.sk, bt = bk / g.kv_heads, hk = bk - bt * g.kv_heads;
+            const int64_t first = (bt * g.heads + hk * g.group) * per + row * g.d + c;
+            f32x4 x = zero, y = zero;
+            for (int p = 0; p < g.q_splits; p++) {
+                x = sum_of(g.part_k + first + p * all, per, g.group, n, vec, x);
+                y = sum_of(g.part_v + first + p * all, per, g.group, n, vec, y);
+            }
+            put(g.dk + bt * g.ks[0] + hk * g.ks[1] + row * g.ks[2] + c, x, n, vec && g.vec_k);
+            put(g.dv + bt * g.vs[0] + hk * g.vs[1] + row * g.vs[2] + c, y, n, vec && g.vec_v);
         }
     }
 }
@@ -1110,9 +1200,8 @@ static int g_force_rows = -1, g_force_splits = 0;
 // Parts into which the walk of `wgs` workgroups is cut, `each` of which share one of the 256 compute units: the longest walk has
 // `longest` steps, `mean` is the average.  Where all are alike the rounds of workgroups count, else (longest first) the longest
 // walk or all the work spread evenly.  A part's start counts as `start` steps, joining as `join` a part.
-// Backward, us, head size 64, causal, whole / in parts as chosen: 64 queries of 8 heads over 4096 keys 303 / 68, 16 heads of 512
-// 122 / 64, of 2048 365 / 284; 128 heads of 1024 491 in one part, 578 in two.  Forward: 64 sequences of one query over 8001 keys
-// 187 / 52, 16 heads of 2048 106 / 83; 64 heads of 256 23 in one part, 39 in two.
+// Us whole / in parts as chosen, head size 64: 64 sequences of one query over 8001 keys 187 / 52, 16 heads of 2048 106 / 83; 64
+// heads of 256 23 in one part, 39 in two.
 static int parts_for(int64_t wgs, int64_t longest, double mean, int each, int start, double join, int most) {
     if (g_force_splits > 0) return (int)(g_force_splits < longest ? g_force_splits : longest > 0 ? longest : 1);
     const int64_t slots = 256 * each;
@@ -1180,21 +1269,54 @@ static int run_forward(RelArgs& g) {
                         "bh_relbias_attention_forward", g);
     }
     if (rc || g.splits == 1) return rc;
-    hipLaunchKernelGGL(relattn_join_kernel, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, stream(), g);
+    hipLaunchKernelGGL(relattn_join_kernel, dim3((unsigned)ceil_div(rows, 16)), dim3(256), 0, stream(), g);
     return BH_LAUNCH_CHECK("bh_relbias_attention_forward: join");
+}
+
+// The same for the backward pass, whose two walks share a launch.  A step over the queries of a key tile (four products) counts
+// 4, one over the keys of a query tile (three) 3; a unit is 0.78 us at head size 64 for a workgroup that has its compute unit to
+// itself, two that share one take 1.45 times as long each.  The longest walk, or all of them spread evenly and what runs last
+// (three quarters of a mean walk, 0.4 where workgroups do not share a unit); parts are written and read at 4 MB in 0.72 us.  The constants are a fit to 13 shapes in 1 to 12
+// parts (within 13 %).  Us whole / in parts as chosen: 8 heads of 64 queries over 4096 keys 298 / 61, 16 heads of 512 69 / 49, 16
+// heads of 2048 248 / 230; 128 heads of 1024 459 in one part, 536 in two, 96 of 128 41 in one, 51 in four.
+struct Walk { int64_t groups, longest; double mean, part_bytes; };
+static void backward_parts(const Walk& keys, const Walk& queries, int each, double size, int& key_parts, int& query_parts) {
+    static const int choices[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32};
+    constexpr double kStart = 0.85, kBytes = 4.3e6;
+    const double last = each == 2 ? 0.75 : 0.4;
+    double least = INFINITY;
+    for (int sk : choices)
+        for (int sq : choices) {
+            if ((sk > 1 && sk > keys.longest) || (sq > 1 && sq > queries.longest)) continue;
+            const double a = 4 * ((double)ceil_div(keys.longest, sk) + kStart), b = 3 * ((double)ceil_div(queries.longest, sq) + kStart);
+            const double am = 4 * (keys.mean / sk + kStart), bm = 3 * (queries.mean / sq + kStart);
+            const double even = ((double)keys.groups * sk * am + (double)queries.groups * sq * bm) / (256.0 * each) * (each == 2 ? 1.45 : 1.0) +
+                                last * (am < bm ? am : bm);
+            const double walks = even > a ? (even > b ? even : b) : a > b ? a : b;
+            const double parts = (sk > 1 ? keys.part_bytes * sk : 0.0) + (sq > 1 ? queries.part_bytes * sq : 0.0);
+            const double cost = walks + parts / (kBytes * size);
+            if (cost < 0.96 * least) { least = cost; key_parts = sk; query_parts = sq; }
+        }
+    if (g_force_splits > 0) {
+        key_parts = (int)(g_force_splits < keys.longest ? g_force_splits : keys.longest > 0 ? keys.longest : 1);
+        query_parts = (int)(g_force_splits < queries.longest ? g_force_splits : queries.longest > 0 ? queries.longest : 1);
+    }
 }
 
 template <int DP>
 static int run_backward(RelArgs& g, float* dtable, int accumulate) {
-    static bool raised_q = false, raised_k = false;
+    static bool raised = false;
     const int64_t nbh = (int64_t)g.batch * g.heads, rows = nbh * g.sq, wgs = (int64_t)g.q_tiles * nbh;
     const int k_tiles = (int)ceil_div(g.sk, 128), each = DP <= 64 ? 2 : 1;
     // dQ walks over a tile's keys, dK and dV over the queries that see one
     const int64_t k_steps = ceil_div(g.sk, 32), q_steps = ceil_div(g.sq, 32);
     const double pairs = seen_pairs(g);
-    g.keys_per_split = ceil_div(k_steps > 0 ? k_steps : 1, parts_for(wgs, k_steps, pairs / (32.0 * g.sq), each, 5, 0, 32)) * 32;
+    int key_parts = 1, query_parts = 1;
+    backward_parts({k_tiles * nbh, q_steps, g.sk > 0 ? pairs / (32.0 * g.sk) : 0.0, 16.0 * nbh * g.sk * g.d},
+                   {wgs, k_steps, pairs / (32.0 * g.sq), 8.0 * rows * g.d}, each, DP / 64.0, key_parts, query_parts);
+    g.keys_per_split = ceil_div(k_steps > 0 ? k_steps : 1, query_parts) * 32;
     g.splits = g.sk > 0 ? (int)ceil_div(g.sk, g.keys_per_split) : 1;
-    g.queries_per_split = (int)ceil_div(q_steps, parts_for(k_tiles * nbh, q_steps, g.sk > 0 ? pairs / (32.0 * g.sk) : 0.0, each, 5, 0, 32)) * 32;
+    g.queries_per_split = (int)ceil_div(q_steps, key_parts) * 32;
     g.q_splits = (int)ceil_div(g.sq, g.queries_per_split);
     Scratch delta, table, planes, part_q, part_kv;
     if (!delta.get(sizeof(float) * (size_t)rows) || !table.get(sizeof(double) * (size_t)g.splits * (size_t)wgs * (size_t)g.buckets)) return BH_ENOMEM;
@@ -1227,16 +1349,21 @@ static int run_backward(RelArgs& g, float* dtable, int accumulate) {
     p.last().dots = g.delta;
     int rc = p.launch<DP>(g.d);
     if (rc) return rc;
-    rc = launch_lds(&relattn_dq_kernel<DP>, raised_q, dim3((unsigned)wgs, (unsigned)g.splits), QueryLds<DP>::BYTES, "bh_relbias_attention_backward: dq", g);
-    if (rc) return rc;
-    if (g.sk > 0) {
-        rc = launch_lds(&relattn_dkv_kernel<DP>, raised_k, dim3((unsigned)(k_tiles * nbh), (unsigned)g.q_splits), KeyLds<DP>::BYTES,
-                        "bh_relbias_attention_backward: dk, dv", g);
+    constexpr int lds = KeyLds<DP>::BYTES > QueryLds<DP>::BYTES ? KeyLds<DP>::BYTES : QueryLds<DP>::BYTES;
+    if (!raised) {
+        rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(&relattn_backward_kernel<DP>), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
+                       "bh_relbias_attention_backward: LDS size");
         if (rc) return rc;
+        raised = true;
     }
-    const auto blocks = [](int64_t n) { const int64_t b = ceil_div(n, 256); return (int)(b < 4096 ? b : 4096); };
-    const Fold f = {(int)ceil_div(g.buckets, 16) * g.heads, g.splits > 1 ? blocks(rows * g.d) : 0,
-                    g.part_k ? blocks((int64_t)g.batch * g.kv_heads * g.sk * g.d) : 0, dtable, accumulate};
+    const int64_t groups = k_tiles * nbh * g.q_splits + wgs * g.splits;
+    hipLaunchKernelGGL(relattn_backward_kernel<DP>, dim3((unsigned)groups), dim3(kThreads), lds, stream(), g, (int)(k_tiles * nbh), (int)wgs);
+    rc = BH_LAUNCH_CHECK("bh_relbias_attention_backward");
+    if (rc) return rc;
+    const int per_block = g.d <= 64 ? 16 : 8;
+    const auto blocks = [&](int64_t n) { const int64_t b = ceil_div(n, per_block); return (int)(b < 4096 ? b : 4096); };
+    const Fold f = {(int)ceil_div(g.buckets, 16) * g.heads, g.splits > 1 ? blocks(rows) : 0,
+                    g.part_k ? blocks((int64_t)g.batch * g.kv_heads * g.sk) : 0, dtable, accumulate};
     hipLaunchKernelGGL(relattn_fold_kernel, dim3((unsigned)(f.table_blocks + f.q_blocks + f.k_blocks)), dim3(256), 0, stream(), g, f);
     return BH_LAUNCH_CHECK("bh_relbias_attention_backward: fold");
 }
