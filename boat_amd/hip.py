@@ -82,6 +82,7 @@ _SIGS = {
     "bh_gemm_force_config": (I, [I]), "bh_gemm_force_direct": (I, [I]), "bh_gemm_force_splits": (I, [I]),
     "bh_gemm_epilogue": (I, [I, I, L, L, L, P, L, P, L, P, L, P, I, P, L, P, L]),
     "bh_dense_act_backward": (I, [I, P, P, P, P, P, P, P, L, L, L, I]),
+    "bh_dense_act_backward_force": (I, [I]),
     "bh_gemm_epilogue_force": (I, [I, I]),
     "bh_transpose_last2": (I, [P, P, L, L, L]),
     "bh_dense_backward": (I, [P, P, P, P, P, P, L, L, L, I]),

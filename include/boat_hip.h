@@ -410,6 +410,8 @@ int bh_relbias_attention_force_splits(int splits);
 /* bh_gemm_epilogue_force: variant 0 = 256x256, 1 = 128x128 tiles through LDS, 2 = 32x32, 3 = 64x64, 4 = 32x32 with sixteen
  * wavefronts (small problems), -1 = by shape (default); splits > 0: cut the contraction this many ways, 0 = by shape */
 int bh_gemm_epilogue_force(int variant, int splits);
+/* bh_dense_act_backward_force: 1 = dx and gw in one launch, 0 = in two, -1 = by shape (default) */
+int bh_dense_act_backward_force(int pair);
 /* bh_sdpa_force_wide: 1 = the attention backward's 256-key workgroups (eight wavefronts) wherever that form exists
  * (head_dim 32 and 64), 0 = never, -1 = chosen by shape (the default) */
 int bh_sdpa_force_wide(int mode);

@@ -224,6 +224,30 @@ def test_dense_backward(hip, rng, act, m, k, n):
     assert np.array_equal(gx.numpy(), first[0])
 
 
+@pytest.mark.parametrize("pair", [0, 1])
+@pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 5, 3), (40, 33, 70), (333, 130, 65), (700, 260, 300)])
+def test_dense_backward_in_one_launch_and_in_two(hip, rng, pair, m, k, n):
+    """dx and dW of a linear layer; either may be left out, and the other keeps its bits."""
+    x, w, dy = (rng.standard_normal(s).astype(np.float32) for s in ((m, k), (k, n), (m, n)))
+    dx_, dw_, ddy = dev(hip, x), dev(hip, w), dev(hip, dy)
+    hip.check(hip.bh_dense_act_backward_force(pair))
+    try:
+        gx, gw = dev(hip, np.full((m, k), np.nan, np.float32)), dev(hip, np.full((k, n), np.nan, np.float32))
+        hip.check(hip.bh_dense_act_backward(-1, ptr(dx_), ptr(dw_), None, ptr(ddy), ptr(gx), ptr(gw), None, m, k, n, 0))
+        alone = dev(hip, np.full((m, k), np.nan, np.float32)), dev(hip, np.full((k, n), np.nan, np.float32))
+        hip.check(hip.bh_dense_act_backward(-1, None, ptr(dw_), None, ptr(ddy), ptr(alone[0]), None, None, m, k, n, 0))
+        hip.check(hip.bh_dense_act_backward(-1, ptr(dx_), None, None, ptr(ddy), None, ptr(alone[1]), None, m, k, n, 0))
+        assert np.array_equal(gx.numpy(), alone[0].numpy()) and np.array_equal(gw.numpy(), alone[1].numpy())
+        hip.check(hip.bh_dense_act_backward(-1, ptr(dx_), ptr(dw_), None, ptr(ddy), ptr(gx), ptr(alone[1]), None, m, k, n, 1))
+    finally:
+        hip.check(hip.bh_dense_act_backward_force(-1))
+    x64, w64, d64 = x.astype(np.float64), w.astype(np.float64), dy.astype(np.float64)
+    bw = oc.product_bound(x64.T, d64)
+    assert (np.abs(gx.numpy() - d64 @ w64.T) <= oc.product_bound(d64, w64.T)).all()
+    assert (np.abs(gw.numpy() - x64.T @ d64) <= bw).all()
+    assert (np.abs(alone[1].numpy() - 2 * (x64.T @ d64)) <= 2 * bw + 2 * oc.U * np.abs(2 * (x64.T @ d64))).all()
+
+
 @pytest.mark.parametrize("act", ["sigmoid", "tanh", "gelu"])
 def test_dense_backward_against_differences(hip, rng, act):
     m, k, n = 9, 20, 7
