@@ -466,7 +466,7 @@ __global__ __launch_bounds__(kSegThreads) void distill_segment_grad_kernel(Disti
 static int distill_check(const char* fn, const float* z, int64_t ldz, const float* teacher, const int32_t* index, int64_t rows, int64_t vocab,
                          int64_t topk, float temperature, float alpha) {
     if (rows < 0 || vocab < 1 || topk < 0) return set_error(BH_EINVAL, "%s: rows >= 0, vocab >= 1 and topk >= 0 are needed", fn);
-    if (vocab > (1 << 30) || rows > 65535 * (int64_t)32768) return set_error(BH_EINVAL, "%s: too many rows or too large a vocabulary", fn);
+    if (vocab > (1 << 30) || rows > (1 << 22)) return set_error(BH_EINVAL, "%s: too many rows or too large a vocabulary", fn);
     if (topk > kMaxTopk) return set_error(BH_EINVAL, "%s: topk is at most %d", fn, kMaxTopk);
     if (ldz < vocab) return set_error(BH_EINVAL, "%s: leading dimension too small", fn);
     if (!(temperature > 0.f) || !(temperature < INFINITY)) return set_error(BH_EINVAL, "%s: the temperature is a positive number", fn);

@@ -8,6 +8,10 @@
  * Return value: 0 on success, a negative BH_E* code otherwise; bh_last_error() gives the
  * message of the most recent failure.  No entry point falls back to host arithmetic.
  *
+ * The fused training operators (bh_gemm_epilogue, bh_dense_act_backward, bh_distill_*, bh_relbias_attention_*) take work
+ * memory for the length of the call: several threads may call them, a stream capture in progress is refused (BH_EINVAL).
+ * They take device pointers of any allocator; what another stream writes has to be finished before the call.
+ *
  * Each kernel entry point names the reference routine (file:line under the Boat tree)
  * whose arithmetic it replaces.
  */
@@ -174,8 +178,8 @@ int bh_softmax_ce_grad(const float* logits, const int32_t* labels, float* dlogit
  * row without any, or with logits of -inf only, has no teacher part), q = softmax(logits / T) and r = softmax(logits):
  *   row_loss = alpha T^2 sum_j p_j (log p_j - log q[index_j]) + (1 - alpha) (-log r[label]),   loss_out[0] = scale * sum of row_loss
  *   dlogits  = seed * scale * (alpha T (q - p) + (1 - alpha) (r - onehot(label)))
- * Without labels the second term is absent.  0 <= topk <= 4096, T > 0, alpha in [0, 1].  row_loss [rows], stats [3 * rows]
- * and loss_out [1] may be NULL.  bh_distill_backward takes the stats of a forward call on the same arguments and seed (one
+ * Without labels the second term is absent.  0 <= topk <= 4096, T > 0, alpha in [0, 1], at most 2^22 rows and 2^30 entries of
+ * the vocabulary.  row_loss [rows], stats [3 * rows] and loss_out [1] may be NULL.  bh_distill_backward takes the stats of a forward call on the same arguments and seed (one
  * float in device memory, NULL = 1); bh_distill_loss_grad is both passes in one (seed 1), reading the logits once.
  * dlogits may be logits itself (ldd == ld); no other overlap. */
 int bh_distill_forward(const float* logits, int64_t ld, const float* teacher, const int32_t* index, const int32_t* labels,
@@ -317,8 +321,9 @@ int bh_sdpa_backward_cached(const float* q, const float* k, const float* v, cons
  * Operands are [batch, heads, rows, d] by strides of batch, head and row in elements (d contiguous; any order of the three);
  * heads is a multiple of kv_heads, head h reads key head h / (heads / kv_heads); 1 <= d <= 128; 2 to 256 buckets.
  * kv_len [batch] (or NULL) holds the number of valid keys of each sequence, values outside [0, sk] counting as the nearer
- * end: what lies behind them is not read.  causal: a query sees keys with r <= 0 only.  A query that sees no key has out = 0,
- * lse = -inf and no gradient.  lse [batch, heads, sq], dense. */
+ * end: what lies behind them is not read.  causal: a query sees keys with r <= 0 only.  What a
+ * key holds that only this mask or its bucket hides has to be finite: its weight is 0, and 0 times infinity is not.  A query that
+ * sees no key has out = 0, lse = -inf and no gradient.  lse [batch, heads, sq], dense. */
 typedef struct bh_relbias_attention {
     int64_t batch, heads, kv_heads, sq, sk, d;
     int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];

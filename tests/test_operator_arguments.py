@@ -62,6 +62,10 @@ def test_distillation_refusals(change, text):
     refused(hip.bh_distill_backward(*distill_args(**change), ANY, None, ANY, 1 << 40), text)
 
 
+def test_distillation_refuses_more_rows_than_a_launch_holds():
+    refused(hip.bh_distill_forward(*distill_args(rows=(1 << 22) + 1), None, None, ANY), "too many rows")
+
+
 def test_distillation_gradient_refusals():
     refused(hip.bh_distill_loss_grad(*distill_args(), None, None, ANY, 99), "leading")
     refused(hip.bh_distill_loss_grad(*distill_args(), None, None, None, 100), "null")
