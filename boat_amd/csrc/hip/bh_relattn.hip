@@ -171,7 +171,8 @@ struct SplitJob {
 constexpr int kMaxJobs = 4;
 struct SplitJobs { SplitJob j[kMaxJobs]; int first[kMaxJobs + 1]; int d; };   // first: workgroup number at which a job starts
 
-// one block of 32 rows a workgroup: read once, written in the forms asked for
+// one block of 32 rows a workgroup: read once, written in the forms asked for.  Bound by memory: keys and values of 128 heads of
+// 1024 at head size 64 (168 MB read and written) 27 us, all four operands of the backward pass (520 MB) 55 us.
 template <int DP>
 __global__ __launch_bounds__(256) void relattn_split_kernel(SplitJobs a) {
     __shared__ float x[32][DP + 4];
@@ -392,7 +393,9 @@ template <int DP> struct ForwardLds {
 };
 
 // A workgroup owns 128 queries of a head, a wavefront 32 of them, and walks over the keys.  Keys and values have a place in
-// LDS each: the next keys are on their way while the values are worked on and the other way round.
+// LDS each: the next keys are on their way while the values are worked on and the other way round.  Bound by the matrix cores and
+// the exponentials and splits beside them: 128 heads of 1024 x 1024 at head size 64 180 us, 190 TFLOP/s of fp32 products (a large
+// library product in bf16 has 195 to offer at six products each), causal 121 us.
 template <int DP>
 __global__ __launch_bounds__(kThreads, 2) void relattn_forward_kernel(RelArgs g) {
     using L = ForwardLds<DP>;
@@ -466,7 +469,7 @@ __global__ __launch_bounds__(kThreads, 2) void relattn_forward_kernel(RelArgs g)
 }
 
 // ---- few query rows (of all the heads that share a key head together) over many keys: wavefronts split the keys, each reads
-// its keys and values once, straight into fragments
+// its keys and values once, straight into fragments.  One query of 64 heads over 8001 keys: 48 us, 5.4 TB/s.
 constexpr int kRowWaves = 4;
 template <int DP>
 __global__ __launch_bounds__(64 * kRowWaves, DP <= 96 ? 2 : 1) void relattn_rows_kernel(RelArgs g, int row_tiles) {
@@ -993,7 +996,9 @@ __device__ __forceinline__ void key_tile(const RelArgs& g, int id, int part) {
 }
 
 // Both walks in one launch: the key tiles, which take longer, first, and the query tiles fill up behind them (one launch after the
-// other, us: 128 heads of 1024, causal, 482 against 459; 32 heads of 1024 at head size 128 379 against 261)
+// other, us: 128 heads of 1024, causal, 482 against 459; 32 heads of 1024 at head size 128 379 against 261).  Bound by the matrix
+// cores at seven products of a head's size (scores and dP are made in both walks: adding up dQ over the key tiles instead would
+// write and read it once per tile): 128 heads of 1024, causal, 410 us, 147 TFLOP/s.
 template <int DP>
 __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_backward_kernel(RelArgs g, int key_groups, int query_groups) {
     const int all_keys = key_groups * g.q_splits, id = blockIdx.x;
@@ -1281,9 +1286,10 @@ static int run_forward(RelArgs& g) {
 // The same for the backward pass, whose two walks share a launch.  A step over the queries of a key tile (four products) counts
 // 4, one over the keys of a query tile (three) 3; a unit is 0.78 us at head size 64 for a workgroup that has its compute unit to
 // itself, two that share one take 1.45 times as long each.  The longest walk, or all of them spread evenly and what runs last
-// (three quarters of a mean walk, 0.4 where workgroups do not share a unit); parts are written and read at 4 MB in 0.72 us.  The constants are a fit to 13 shapes in 1 to 12
-// parts (within 13 %).  Us whole / in parts as chosen: 8 heads of 64 queries over 4096 keys 298 / 61, 16 heads of 512 69 / 49, 16
-// heads of 2048 248 / 230; 128 heads of 1024 459 in one part, 536 in two, 96 of 128 41 in one, 51 in four.
+// (three quarters of a mean walk, 0.4 where workgroups do not share a unit); parts are written and read at 4 MB in 0.72 us.  The
+// constants are a fit to 13 shapes in 1 to 12 parts (within 13 %).  Us whole / in parts as chosen: 8 heads of 64 queries over 4096
+// keys 298 / 61, 16 heads of 512 69 / 49, 16 heads of 2048 248 / 230; 128 heads of 1024 459 in one part, 536 in two, 96 of 128 41
+// in one, 51 in four.
 struct Walk { int64_t groups, longest; double mean, part_bytes; };
 static void backward_parts(const Walk& keys, const Walk& queries, int each, double size, int& key_parts, int& query_parts) {
     static const int choices[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32};
