@@ -651,6 +651,7 @@ int bh_gemm_epilogue(int trans_a, int trans_b, int64_t m, int64_t n, int64_t k, 
     BH_CHECK_ARG(c && ((a && b) || k == 0), "null pointer");
     BH_CHECK_ARG(lda >= (trans_a ? m : k) && ldb >= (trans_b ? k : n) && ldc >= n, "leading dimension too small");
     BH_CHECK_ARG((!saved || lds >= n) && (!residual || ldr >= n), "leading dimension too small");
+    BH_CHECK_ARG(residual != c || ldr == ldc, "a residual in place has the output's leading dimension");
     BH_REQUIRE_INIT();
     BH_CALL_GUARD();
     ProfScope prof(BH_PROF_GEMM, 2.0 * (double)m * (double)n * (double)k);

@@ -666,3 +666,39 @@ def test_capture_is_refused(hip):
             rt.hipGraphDestroy(graph)
     assert rcs == [-1, -1, -1] and "captured" in text
     assert (d.numpy() == 1).all()
+
+
+def test_attention_and_distillation_from_several_threads(hip, rng):
+    """Work memory of one call is not another's: the same inputs give the same bits from every thread."""
+    q, k, v, table, d_out = attention_case(rng, 2, 4, 2, 70, 300, 48, 16)
+    strides = [(a.shape[1] * a.shape[2] * a.shape[3], a.shape[2] * a.shape[3], a.shape[3]) for a in (q, k, v, q)]
+    plan = hip.relbias_attention(batch=2, heads=4, kv_heads=2, sq=70, sk=300, d=48, q_stride=strides[0], k_stride=strides[1], v_stride=strides[2],
+                                 o_stride=strides[3], query_offset=230, num_buckets=16, max_distance=64, bidirectional=0, causal=1, scale=0.2)
+    dq, dk, dv, dt, dd = (dev(hip, a) for a in (q, k, v, table, d_out))
+    z, teacher, index, labels = distill_case(rng, 5, 20001, 7)
+    dz, de, di, dy = (dev(hip, a) for a in (z, teacher, index, labels))
+    rcs = []
+
+    def outputs():
+        return [dev(hip, np.full(s, np.nan, np.float32)) for s in (q.shape, (2, 4, 70), q.shape, k.shape, v.shape, table.shape, z.shape, (1,))]
+
+    def call(o):
+        for _ in range(5):
+            rcs.append(hip.bh_relbias_attention_forward(plan, ptr(dq), ptr(dk), ptr(dv), ptr(dt), None, ptr(o[0]), ptr(o[1])))
+            rcs.append(hip.bh_relbias_attention_backward(plan, ptr(dq), ptr(dk), ptr(dv), ptr(dt), None, ptr(o[0]), ptr(o[1]), ptr(dd), ptr(o[2]),
+                                                         ptr(o[3]), ptr(o[4]), ptr(o[5]), 0))
+            rcs.append(hip.bh_distill_loss_grad(ptr(dz), 20001, ptr(de), ptr(di), ptr(dy), 5, 20001, 7, 2.0, 0.5, 0.2, None, ptr(o[7]), ptr(o[6]), 20001))
+    first = outputs()
+    call(first)
+    want = [x.numpy() for x in first]
+    assert all(np.isfinite(x).all() for x in want)
+    outs = [outputs() for _ in range(4)]
+    threads = [threading.Thread(target=call, args=(o,)) for o in outs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert rcs == [0] * 75
+    for o in outs:
+        for x, w in zip(o, want):
+            assert np.array_equal(x.numpy(), w)

@@ -62,6 +62,15 @@ def test_distillation_refusals(change, text):
     refused(hip.bh_distill_backward(*distill_args(**change), ANY, None, ANY, 1 << 40), text)
 
 
+def test_a_residual_in_place_has_the_outputs_rows():
+    refused(gemm(residual=ANY, ldr=5), "in place")
+
+
+@pytest.mark.parametrize("temperature", [2e19, 1e-39, 3e38])
+def test_distillation_refuses_temperatures_out_of_range(temperature):
+    refused(hip.bh_distill_forward(*distill_args(temperature=temperature), None, None, ANY), "temperature")
+
+
 def test_distillation_refuses_more_rows_than_a_launch_holds():
     refused(hip.bh_distill_forward(*distill_args(rows=(1 << 22) + 1), None, None, ANY), "too many rows")
 
