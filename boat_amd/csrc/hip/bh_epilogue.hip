@@ -27,6 +27,7 @@ struct EpiArgs {
     int splits;                              // > 1: partial sums go to `partial` [split][m][n], epilogue_fold_kernel finishes
     int64_t k_per_split;                     // multiple of 16
     float* partial;
+    float* colsum; int colsum_add;           // small tiles, both operands along rows: [n] (+)= column sums of B, or NULL
 };
 
 __device__ __forceinline__ float act_value(int act, float z) {
@@ -426,6 +427,12 @@ __device__ __forceinline__ void small_tile(const EpiArgs& g, int tile, int split
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
     // kDepth steps' loads are issued before the first one's products
     constexpr int kDepth = T == 1 && WAVES == 8 ? 2 : 1, kStep = 16 * WAVES;
+    // a layer's bias gradient rides with its weight gradient: the first tile row's workgroups add up what they read of dz
+    constexpr bool kSums = !A_KC && !B_KC;
+    const bool wants = kSums && g.colsum && m0 == 0;
+    float column[T];
+#pragma unroll
+    for (int i = 0; i < T; i++) column[i] = 0.f;
     const int64_t half = 8 * (lane >> 5);
     for (int64_t k = kb + 16 * wave; k < ke; k += kDepth * kStep) {
         float x[kDepth][T][8], y[kDepth][T][8];
@@ -438,6 +445,12 @@ __device__ __forceinline__ void small_tile(const EpiArgs& g, int tile, int split
             }
 #pragma unroll
         for (int d = 0; d < kDepth; d++) {
+            if constexpr (kSums)
+                if (wants) {
+#pragma unroll
+                    for (int i = 0; i < T; i++)
+                        column[i] += ((y[d][i][0] + y[d][i][1]) + (y[d][i][2] + y[d][i][3])) + ((y[d][i][4] + y[d][i][5]) + (y[d][i][6] + y[d][i][7]));
+                }
             u32x4 fa[T][kPlanes], fb[T][kPlanes];
 #pragma unroll
             for (int i = 0; i < T; i++) { split_eight(x[d][i], fa[i]); split_eight(y[d][i], fb[i]); }
@@ -467,6 +480,22 @@ __device__ __forceinline__ void small_tile(const EpiArgs& g, int tile, int split
                     if (!finite_f32(s)) s = plain_element<A_KC, B_KC>(g, r, c, 0, g.k);
                     finish_element(g, r, c, s);
                 }
+            }
+        }
+    if constexpr (kSums)
+        if (wants) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < T; i++) {
+                const float both = column[i] + __shfl_xor(column[i], 32, 64);
+                if (lane < 32) sums[wave][32 * i + lane] = both;
+            }
+            __syncthreads();
+            if (tid < 32 * T && n0 + tid < g.n) {
+                float t = 0.f;
+#pragma unroll
+                for (int w = 0; w < WAVES; w++) t += sums[w][tid];
+                g.colsum[n0 + tid] = g.colsum_add ? g.colsum[n0 + tid] + t : t;
             }
         }
 }
@@ -597,13 +626,14 @@ static double choose(int64_t m, int64_t n, int64_t k, int along_rows, int& varia
     return best;
 }
 
-static int product(int trans_a, int trans_b, EpiArgs g) {
+static void pick(int trans_a, int trans_b, const EpiArgs& g, int& variant, int& splits) {
     constexpr int64_t kMaxLd = (int64_t)1 << 22;   // 256 rows of a tile within 32 bits of bytes; past it the small tiles' addresses
-    int variant, splits;
     choose(g.m, g.n, g.k, (trans_a ? 1 : 0) + (trans_b ? 0 : 1), variant, splits);
     if (g_force_variant >= 0) { variant = g_force_variant; splits = 1; }
     if (g_force_splits > 0) splits = g_force_splits;
     if (variant <= kTile128 && (g.lda >= kMaxLd || g.ldb >= kMaxLd)) { variant = kSmall64; splits = 1; }
+}
+static int product(int trans_a, int trans_b, const EpiArgs& g, int variant, int splits) {
     if (!trans_a) return trans_b ? run_product<true, true>(g, variant, splits) : run_product<true, false>(g, variant, splits);
     return trans_b ? run_product<false, true>(g, variant, splits) : run_product<false, false>(g, variant, splits);
 }
@@ -658,7 +688,9 @@ int bh_gemm_epilogue(int trans_a, int trans_b, int64_t m, int64_t n, int64_t k, 
     EpiArgs g = {};
     g.a = a; g.b = b; g.m = m; g.n = n; g.k = k; g.lda = lda; g.ldb = ldb; g.c = c; g.ldc = ldc; g.bias = bias;
     g.saved = saved; g.lds = lds; g.residual = residual; g.ldr = ldr; g.act = act;
-    return product(trans_a, trans_b, g);
+    int variant, splits;
+    pick(trans_a, trans_b, g, variant, splits);
+    return product(trans_a, trans_b, g, variant, splits);
 }
 
 int bh_dense_act_backward(int act, const float* x, const float* w, const float* saved, const float* dy, float* dx, float* gw, float* gb,
@@ -668,34 +700,45 @@ int bh_dense_act_backward(int act, const float* x, const float* w, const float* 
     BH_CHECK_ARG((dy && (!dx || w) && (!gw || x) && (act == BH_ACT_NONE || saved)) || m == 0 || n == 0, "null pointer");
     BH_REQUIRE_INIT();
     BH_CALL_GUARD();
-    // dz = dy * act'(z), and with it db = its column sums
+    EpiArgs a = {}, b = {};                                   // dx[m,k] = dz[m,n] . w[k,n]^T,  gw[k,n] (+)= x[m,k]^T . dz[m,n]
+    a.b = w; a.lda = n; a.ldb = n; a.c = dx; a.ldc = k; a.m = m; a.n = k; a.k = n; a.act = BH_ACT_NONE;
+    b.a = x; b.lda = k; b.ldb = n; b.c = gw; b.ldc = n; b.m = k; b.n = n; b.k = m; b.act = BH_ACT_NONE;
+    b.residual = accumulate ? gw : nullptr; b.ldr = n;
+    const bool whole = m > 0 && k > 0 && n > 0, one = whole && (dx || gw) && in_one_launch(m, k, n);
+    int variant = kSmallLong, splits = 1;
+    if (gw && whole && !one) pick(1, 0, b, variant, splits);
+    // db = the column sums of dz: with dW where small tiles make that whole, else with dz (or alone)
+    const bool rides = gb && gw && whole && variant >= kSmall32 && splits == 1;
+    if (rides) { b.colsum = gb; b.colsum_add = accumulate ? 1 : 0; }
+    // dz = dy * act'(z)
     const float* dz = dy;
     Scratch own;
     int rc = BH_OK;
     if (act != BH_ACT_NONE && m > 0 && n > 0 && (dx || gw || gb)) {
         if (!own.get(sizeof(float) * (size_t)(m * n))) return BH_ENOMEM;
-        rc = gb ? bh_activation_backward_colsum(act, saved, dy, (float*)own.p, gb, m, n, accumulate)
-                : bh_activation_backward(act, saved, dy, (float*)own.p, m * n, 0);
+        rc = gb && !rides ? bh_activation_backward_colsum(act, saved, dy, (float*)own.p, gb, m, n, accumulate)
+                          : bh_activation_backward(act, saved, dy, (float*)own.p, m * n, 0);
         dz = (const float*)own.p;
-    } else if (gb && n > 0) {
+    } else if (gb && n > 0 && !rides) {
         rc = m > 0 ? bh_colsum(dy, gb, m, n, accumulate) : accumulate ? BH_OK : bh_fill(gb, 0.f, n);
     }
     if (rc != BH_OK) return rc;
-    if (m > 0 && k > 0 && n > 0 && (dx || gw) && in_one_launch(m, k, n)) {
+    a.a = dz;
+    b.b = dz;
+    if (one) {
         // also for one of the two: its bits do not depend on whether the other is asked for
         ProfScope prof(BH_PROF_GEMM, (dx && gw ? 4.0 : 2.0) * (double)m * (double)n * (double)k);
-        EpiArgs a = {}, b = {};
-        if (dx) { a.a = dz; a.lda = n; a.b = w; a.ldb = n; a.c = dx; a.ldc = k; a.m = m; a.n = k; a.k = n; a.act = BH_ACT_NONE; }
-        if (gw) { b.a = x; b.lda = k; b.b = dz; b.ldb = n; b.c = gw; b.ldc = n; b.m = k; b.n = n; b.k = m; b.act = BH_ACT_NONE; }
-        b.residual = accumulate ? gw : nullptr; b.ldr = n;
+        if (!dx) a.m = 0;
+        if (!gw) b.m = 0;
         return launch_pair(a, b, n % 4 == 0 && aligned16(dz), n % 4 == 0 && aligned16(w));
     }
-    // dx[m,k] = dz[m,n] . w[k,n]^T     (n == 0: zeros)
+    // n == 0: zeros
     if (dx) rc = bh_gemm_epilogue(0, 1, m, k, n, dz, n, w, n, dx, k, nullptr, BH_ACT_NONE, nullptr, 0, nullptr, 0);
-    // gw[k,n] (+)= x[m,k]^T . dz[m,n]  (m == 0: zeros)
-    if (rc == BH_OK && gw)
-        rc = bh_gemm_epilogue(1, 0, k, n, m, x, k, dz, n, gw, n, nullptr, BH_ACT_NONE, nullptr, 0, accumulate ? gw : nullptr, n);
-    return rc;
+    if (rc != BH_OK || !gw) return rc;
+    // m == 0: zeros
+    if (!whole) return bh_gemm_epilogue(1, 0, k, n, m, x, k, dz, n, gw, n, nullptr, BH_ACT_NONE, nullptr, 0, accumulate ? gw : nullptr, n);
+    ProfScope prof(BH_PROF_GEMM, 2.0 * (double)m * (double)n * (double)k);
+    return product(1, 0, b, variant, splits);
 }
 
 int bh_gemm_epilogue_force(int variant, int splits) {

@@ -224,6 +224,34 @@ def test_dense_backward(hip, rng, act, m, k, n):
     assert np.array_equal(gx.numpy(), first[0])
 
 
+@pytest.mark.parametrize("variant,splits,pair", [(0, 1, 0), (1, 3, 0), (2, 1, 0), (3, 1, 0), (3, 2, 0), (4, 1, 0), (-1, 0, 1)])
+@pytest.mark.parametrize("m,k,n", [(1, 1, 1), (40, 33, 70), (700, 100, 300), (270, 513, 65)])
+def test_bias_gradient_with_and_without_the_weights(hip, rng, variant, splits, pair, m, k, n):
+    x, w, dy = (rng.standard_normal(s).astype(np.float32) for s in ((m, k), (k, n), (m, n)))
+    z = rng.standard_normal((m, n)).astype(np.float32)
+    dx_, dw_, ddy, dz_ = (dev(hip, a) for a in (x, w, dy, z))
+    slope = (dy * (z > 0)).astype(np.float64)
+    hip.check(hip.bh_gemm_epilogue_force(variant, splits))
+    hip.check(hip.bh_dense_act_backward_force(pair))
+    try:
+        for act, want in ((-1, dy.astype(np.float64)), (0, slope)):
+            bound = 2 * m * oc.U * np.abs(want).sum(0)
+            for weights in (True, False):
+                gw, gb = dev(hip, np.full((k, n), np.nan, np.float32)), dev(hip, np.full(n, np.nan, np.float32))
+                gx = dev(hip, np.full((m, k), np.nan, np.float32))
+                call = (act, ptr(dx_), ptr(dw_), ptr(dz_), ptr(ddy), ptr(gx), ptr(gw) if weights else None, ptr(gb), m, k, n)
+                hip.check(hip.bh_dense_act_backward(*call, 0))
+                first = gb.numpy()
+                assert (np.abs(first - want.sum(0)) <= bound).all()
+                hip.check(hip.bh_dense_act_backward(*call, 1))
+                assert (np.abs(gb.numpy() - 2 * first.astype(np.float64)) <= 2 * bound + 4 * oc.U * np.abs(first)).all()
+                assert not weights or (np.abs(gw.numpy() - 2 * (x.T.astype(np.float64) @ want)) <=
+                                       4 * oc.product_bound(x.T.astype(np.float64), want) + 1e-30).all()
+    finally:
+        hip.check(hip.bh_gemm_epilogue_force(-1, 0))
+        hip.check(hip.bh_dense_act_backward_force(-1))
+
+
 @pytest.mark.parametrize("pair", [0, 1])
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 5, 3), (40, 33, 70), (333, 130, 65), (700, 260, 300)])
 def test_dense_backward_in_one_launch_and_in_two(hip, rng, pair, m, k, n):
