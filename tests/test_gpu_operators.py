@@ -730,3 +730,78 @@ def test_attention_and_distillation_from_several_threads(hip, rng):
     for o in outs:
         for x, w in zip(o, want):
             assert np.array_equal(x.numpy(), w)
+
+
+FAR = (1 << 30) + 64                                         # floats between rows or sequences: three of them pass 2^32 bytes
+
+
+@pytest.fixture(scope="module")
+def far(hip):
+    """One buffer that rows and sequences lie far apart in; put() and get() move rows of it."""
+    whole = hip.empty((3 * FAR,))
+
+    class Far:
+        @staticmethod
+        def at(offset=0):
+            return C.c_void_p(whole.ptr + 4 * offset)
+
+        @staticmethod
+        def put(offset, rows):
+            for i, row in enumerate(rows):
+                row = np.ascontiguousarray(row, dtype=np.float32)
+                hip.check(hip.bh_memcpy_h2d(whole.ptr + 4 * (offset + i * FAR), row.ctypes.data, row.nbytes))
+
+        @staticmethod
+        def get(offset, shape):
+            out = np.empty(shape, np.float32)
+            for i in range(shape[0]):
+                part = np.empty(shape[1:], np.float32)
+                hip.check(hip.bh_memcpy_d2h(part.ctypes.data, whole.ptr + 4 * (offset + i * FAR), part.nbytes))
+                out[i] = part
+            return out
+    yield Far
+
+
+def test_product_rows_far_apart(hip, rng, far):
+    a, b, r = (rng.standard_normal(s).astype(np.float32) for s in ((3, 100), (100, 70), (3, 70)))
+    far.put(0, a)
+    far.put(1000, r)
+    hip.check(hip.bh_gemm_epilogue(0, 0, 3, 70, 100, far.at(0), FAR, ptr(dev(hip, b)), 70, far.at(2000), FAR, None, -1, far.at(3000), FAR,
+                                   far.at(1000), FAR))
+    z, bound = a.astype(np.float64) @ b, oc.product_bound(a.astype(np.float64), b.astype(np.float64))
+    assert (np.abs(far.get(3000, (3, 70)) - z) <= bound).all()
+    assert (np.abs(far.get(2000, (3, 70)) - z - r) <= bound + 2 * oc.U * np.abs(z + r)).all()
+
+
+def test_distill_rows_far_apart(hip, rng, far):
+    z, teacher, index, labels = distill_case(rng, 3, 1000, 6)
+    want_row, want_loss, want_dz = oc.distill(z, teacher, index, labels, 2.0, 0.5, 1.0)
+    tol_row, tol_dz = oc.distill_bounds(z, teacher, 2.0, 0.5, 1.0)
+    far.put(0, z)
+    loss = hip.zeros(1)
+    hip.check(hip.bh_distill_loss_grad(far.at(0), FAR, ptr(dev(hip, teacher)), ptr(dev(hip, index)), ptr(dev(hip, labels)), 3, 1000, 6, 2.0, 0.5, 1.0,
+                                       None, ptr(loss), far.at(5000), FAR))
+    assert abs(loss.numpy()[0] - want_loss) <= 3 * tol_row + 4 * oc.U * abs(want_loss)
+    assert (np.abs(far.get(5000, (3, 1000)) - want_dz) <= tol_dz).all()
+
+
+@pytest.mark.parametrize("sq", [1, 40])
+def test_attention_sequences_far_apart(hip, rng, far, sq):
+    """a cache of keys and values whose sequences lie 2^30 floats apart"""
+    q, k, v, table, d_out = attention_case(rng, 3, 2, 1, sq, 90, 32, 16)
+    want, bound = oc.attention(q, k, v, table, None, 90 - sq, 16, 20, False, True, 0.2, d_out)
+    places = {n: 100000 * i for i, n in enumerate(("q", "k", "v", "out", "d_out", "dq", "dk", "dv"))}
+    for n, x in (("q", q), ("k", k), ("v", v), ("d_out", d_out)):
+        far.put(places[n], x)
+    at = {n: far.at(o) for n, o in places.items()}
+    plan = hip.relbias_attention(batch=3, heads=2, kv_heads=1, sq=sq, sk=90, d=32, q_stride=(FAR, sq * 32, 32), k_stride=(FAR, 90 * 32, 32),
+                                 v_stride=(FAR, 90 * 32, 32), o_stride=(FAR, sq * 32, 32), query_offset=90 - sq, num_buckets=16, max_distance=20,
+                                 bidirectional=0, causal=1, scale=0.2)
+    dt, lse, gt = dev(hip, table), hip.empty((3, 2, sq)), hip.empty(table.shape)
+    hip.check(hip.bh_relbias_attention_forward(plan, at["q"], at["k"], at["v"], ptr(dt), None, at["out"], ptr(lse)))
+    hip.check(hip.bh_relbias_attention_backward(plan, at["q"], at["k"], at["v"], ptr(dt), None, at["out"], ptr(lse), at["d_out"], at["dq"], at["dk"],
+                                                at["dv"], ptr(gt), 0))
+    got = {n: far.get(places[n], x.shape) for n, x in (("out", q), ("dq", q), ("dk", k), ("dv", v))}
+    got["dtable"], got["lse"] = gt.numpy(), lse.numpy()
+    for n in got:
+        assert (np.abs(got[n] - want[n]) <= bound[n] + 1e-37).all(), n
