@@ -62,7 +62,8 @@ struct RelArgs {
 
 // ---- the bias as a workgroup sees it.  Where the borders span no more than kLine relative positions LDS holds the bias (times
 // log2 e) and the bucket of each of them, worked out once; else the borders and the head's table column, and every wavefront
-// looks its blocks' diagonals up.
+// looks its blocks' diagonals up.  With a line / with lookups, 32 buckets to distance 128, us: 128 heads of 1024 forward 203 / 205,
+// causal with backward 586 / 593; 5 KB of LDS let two workgroups share a compute unit at every head size.
 constexpr int kLine = 1024;
 
 __device__ __forceinline__ int bucket_of(const Buckets& b, const int* border, int rel) {
