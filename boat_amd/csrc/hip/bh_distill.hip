@@ -509,15 +509,15 @@ static void cut_row(DistillArgs& g, int segments) {
 
 template <int THREADS, int NV, int LV, bool GRAD>
 static int launch_row_kernel(const DistillArgs& g) {
-    const size_t bytes = sizeof(float) * (4 * (size_t)LV * THREADS + 3 * (size_t)entry_slots(g.topk));
-    static size_t raised = 64 * 1024;
-    if (bytes > raised) {
+    const auto bytes = [](int topk) { return sizeof(float) * (4 * (size_t)LV * THREADS + 3 * (size_t)entry_slots(topk)); };
+    static bool raised = false;                  // the most that any call needs, so that two threads may both ask for it
+    if (!raised && bytes(kMaxTopk) > 64 * 1024) {
         const int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(&distill_row_kernel<THREADS, NV, LV, GRAD>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "bh_distill: LDS size");
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(kMaxTopk)), "bh_distill: LDS size");
         if (rc) return rc;
-        raised = bytes;
+        raised = true;
     }
-    hipLaunchKernelGGL((distill_row_kernel<THREADS, NV, LV, GRAD>), dim3((unsigned)g.rows), dim3(THREADS), bytes, stream(), g);
+    hipLaunchKernelGGL((distill_row_kernel<THREADS, NV, LV, GRAD>), dim3((unsigned)g.rows), dim3(THREADS), bytes(g.topk), stream(), g);
     return BH_LAUNCH_CHECK("bh_distill");
 }
 

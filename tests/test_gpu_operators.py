@@ -382,6 +382,11 @@ def test_distill_large_vocabularies(hip, rng, rows, vocab, topk):
     check_distill(hip, *distill_case(rng, rows, vocab, topk), 3.0, 0.8, pad=3 if rows < 100 else 0)
 
 
+@pytest.mark.parametrize("rows,vocab", [(2, 900), (2, 1900), (3, 3000), (2, 6000), (2, 16000), (2, 30000), (129, 26000)])
+def test_distill_most_kept_entries(hip, rng, rows, vocab):
+    check_distill(hip, *distill_case(rng, rows, vocab, 4096), 2.0, 0.7)
+
+
 @pytest.mark.parametrize("rows,vocab", [(1, 16387), (127, 16383), (127, 16384), (128, 16384), (70, 40003), (1, 12001)])
 def test_distill_rows_in_segments_and_whole(hip, rng, rows, vocab):
     check_distill(hip, *distill_case(rng, rows, vocab, 11), 2.0, 0.7, pad=1 if rows < 100 else 0)
