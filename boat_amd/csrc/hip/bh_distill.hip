@@ -25,7 +25,7 @@ namespace bh {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // rows of odd length start anywhere
 
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kMaxTopk = 4096;
 
 struct DistillArgs {
@@ -58,27 +58,28 @@ struct RowStats {
     }
 };
 
-// The exponents are fma(z, log2(e)/T, -max log2(e)/T), one rounding each; the rounding of the second product is the same factor
-// in every term and in the sum.  Where T is a small whole number the softmax at 1 takes its terms from the one at T: the
-// exponential is the slowest instruction here (a quarter of the rate of the others).
+// The exponents are (z - max) log2(e)/T, the maximum taken off first: their error is two roundings of themselves, however far
+// the logits lie from zero, and a maximum's own exponent is 0.  (As fma(z, log2(e)/T, -max log2(e)/T) it would be the rounding of
+// the second product, which differs from thread to thread with the maximum and overflows under masks like -1e10.)  Where T is a
+// small whole number the softmax at 1 takes its terms from the one at T: the exponential is the slowest instruction here (a
+// quarter of the rate of the others).
 template <int POWER>
-__device__ __forceinline__ float hard_term(float soft, float z, float off) {
+__device__ __forceinline__ float hard_term(float soft, float below) {
     if (POWER == 1) return soft;
     if (POWER == 2) return soft * soft;
     if (POWER == 3) return soft * soft * soft;
     if (POWER == 4) return (soft * soft) * (soft * soft);
-    return fast_exp2(fmaf(z, kLog2e, off));
+    return fast_exp2(below * kLog2e);
 }
 template <int POWER, bool HARD, int N>
 __device__ __forceinline__ void add_terms(const f32x4 (&v)[N], float b, float cold, float& a, float& c) {
-    const float off = -b * cold, off1 = -b * kLog2e;
 #pragma unroll
     for (int i = 0; i < N; i++) {
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            const float t = fast_exp2(fmaf(v[i][q], cold, off));
+            const float below = v[i][q] - b, t = fast_exp2(below * cold);
             a += t;
-            if (HARD) c += hard_term<POWER>(t, v[i][q], off1);
+            if (HARD) c += hard_term<POWER>(t, below);
         }
         __builtin_amdgcn_sched_barrier(0);   // one vector's temporaries at a time: the registers hold the row
     }
@@ -149,7 +150,7 @@ __device__ __forceinline__ void stats_of_one(float x, float cold, RowStats& s) {
 // ---- the special places of a row: the teacher's entries and, last, the label, staged in LDS
 struct Entries {
     int* index;       // [topk + 1], -1 = left out
-    float* value;     // [topk + 1] teacher logit / T
+    float* value;     // [topk + 1] teacher logit
     float* logit;     // [topk + 1] student logit at the index
 };
 // the indices come first and fill whole vectors of four (-2 behind the label)
@@ -163,7 +164,7 @@ struct Entry {
     __device__ __forceinline__ Entry(const DistillArgs& g, int64_t row, int j) : index(j > g.topk ? -2 : -1), value(-INFINITY) {
         if (j < g.topk) {
             index = g.index[row * g.topk + j];
-            value = g.teacher[row * g.topk + j] * g.inv_t;
+            value = g.teacher[row * g.topk + j];
         } else if (j == g.topk && g.labels) {
             index = g.labels[row];
         }
@@ -184,7 +185,7 @@ __device__ __forceinline__ void teacher_softmax(const DistillArgs& g, const Entr
     m = wave_max(m);
     float s = 0.f;
     if (m > -INFINITY)
-        for (int j = lane; j < g.topk; j += 64) s += fast_exp2((e.value[j] - m) * kLog2e);
+        for (int j = lane; j < g.topk; j += 64) s += fast_exp2((e.value[j] - m) * g.cold);
     s = wave_sum(s);
     top = m;
     inv_sum = s;   // the sum itself: 0 when nothing is kept
@@ -198,12 +199,12 @@ __device__ __forceinline__ float row_loss_of(const DistillArgs& g, const Entries
     if (sum != 0.f) {
         const float ls = logf(sum), lt = logf(s.st), inv = 1.f / sum;
         for (int j = lane; j < g.topk; j += 64) {
-            const float lp = e.value[j] - top, p = fast_exp2(lp * kLog2e) * inv;
-            if (p > 0.f || p != p) acc += p * ((lp - ls) - (fmaf(e.logit[j], g.cold, -b * g.cold) * kLn2 - lt));
+            const float below = e.value[j] - top, p = fast_exp2(below * g.cold) * inv;
+            if (p > 0.f || p != p) acc += p * ((below * g.inv_t - ls) - ((e.logit[j] - b) * g.inv_t - lt));
         }
     }
     acc = wave_sum(acc) * g.w_soft;
-    if (g.w_hard != 0.f && e.index[g.topk] >= 0) acc += g.w_hard * (logf(s.s1) - fmaf(e.logit[g.topk], kLog2e, -b * kLog2e) * kLn2);
+    if (g.w_hard != 0.f && e.index[g.topk] >= 0) acc += g.w_hard * (logf(s.s1) - (e.logit[g.topk] - b));
     return acc;
 }
 
@@ -231,18 +232,18 @@ __global__ __launch_bounds__(1024) void distill_loss_kernel(const float* __restr
     }
 }
 
-struct GradRow { float cold, off, off1, ct, c1; int power; };   // dz = ct exp2(z cold + off) + c1 exp2(z log2 e + off1)
+struct GradRow { float cold, base, ct, c1; int power; };   // dz = ct exp2((z - base) cold) + c1 exp2((z - base) log2 e)
 
 __device__ __forceinline__ GradRow grad_row(const DistillArgs& g, const Entries& e, const RowStats& s, float sum) {
     const float seed = g.seed ? g.seed[0] : 1.f, b = RowStats::base(s.m);
     const bool hard = g.w_hard != 0.f && e.index[g.topk] >= 0;
-    return {g.cold, -b * g.cold, -b * kLog2e, sum != 0.f ? g.g_soft * seed / s.st : 0.f, hard ? g.g_hard * seed / s.s1 : 0.f, g.power};
+    return {g.cold, b, sum != 0.f ? g.g_soft * seed / s.st : 0.f, hard ? g.g_hard * seed / s.s1 : 0.f, g.power};
 }
 // POWER as above; -1: without the softmax at 1
 template <int POWER>
 __device__ __forceinline__ float grad_term(const GradRow& r, float z) {
-    const float t = fast_exp2(fmaf(z, r.cold, r.off)), d = r.ct * t;
-    return POWER < 0 ? d : fmaf(r.c1, hard_term<POWER>(t, z, r.off1), d);
+    const float below = z - r.base, t = fast_exp2(below * r.cold), d = r.ct * t;
+    return POWER < 0 ? d : fmaf(r.c1, hard_term<POWER>(t, below), d);
 }
 // calls f with the power as a constant: which it is holds for the whole launch, so the choice stands outside the loops
 template <typename F>
@@ -284,13 +285,13 @@ __device__ __forceinline__ void grad_entries(const DistillArgs& g, const Entries
             same += (x.x == i) + (x.y == i) + (x.z == i) + (x.w == i);
         }
         bool first = true;
-        float w = j == g.topk ? hard : soft == 0.f ? 0.f : soft * fast_exp2((e.value[j] - top) * kLog2e);
+        float w = j == g.topk ? hard : soft == 0.f ? 0.f : soft * fast_exp2((e.value[j] - top) * g.cold);
         if (same > 1) {
             w = 0.f;
             for (int o = 0; o <= g.topk; o++) {
                 if (e.index[o] != i) continue;
                 if (o < j) { first = false; break; }
-                w += o == g.topk ? hard : soft == 0.f ? 0.f : soft * fast_exp2((e.value[o] - top) * kLog2e);
+                w += o == g.topk ? hard : soft == 0.f ? 0.f : soft * fast_exp2((e.value[o] - top) * g.cold);
             }
         }
         if (first) dz[i] = grad_at(r, g.w_hard != 0.f, e.logit[j]) - w;
