@@ -34,7 +34,7 @@ struct DistillArgs {
     const int32_t* labels;                         // [rows] or NULL
     int64_t rows; int vocab; int topk;
     float cold;                                    // log2(e) / T
-    int power;                                     // T where it is 1, 2, 3 or 4, else 0: exp(x) is then exp(x/T)^T
+    int terms;                                     // which softmaxes a row needs: kSoft, kSame or kBoth
     float inv_t, w_soft, w_hard;                   // 1/T, alpha T^2, 1 - alpha (0 without labels)
     float g_soft, g_hard;                          // scale alpha T, scale (1 - alpha)
     const float* seed;                             // device scalar on the gradient, or NULL
@@ -60,18 +60,15 @@ struct RowStats {
 
 // The exponents are (z - max) log2(e)/T, the maximum taken off first: their error is two roundings of themselves, however far
 // the logits lie from zero, and a maximum's own exponent is 0.  (As fma(z, log2(e)/T, -max log2(e)/T) it would be the rounding of
-// the second product, which differs from thread to thread with the maximum and overflows under masks like -1e10.)  Where T is a
-// small whole number the softmax at 1 takes its terms from the one at T: the exponential is the slowest instruction here (a
-// quarter of the rate of the others).
-template <int POWER>
+// the second product, which differs from thread to thread with the maximum and overflows under masks like -1e10.)  The softmax at 1
+// has exponentials of its own.  (Powers of the ones at T, for whole T, multiply their error by T and save next to
+// nothing: 4096 x 50001 at T = 3 337 us with them, 336 without, 37 x 128001 at T = 2 17.0 and 17.4.)
+enum { kSoft, kSame, kBoth };   // the softmax at T alone (no labels, or no weight on them); T = 1: both are one; two softmaxes
+template <int TERMS>
 __device__ __forceinline__ float hard_term(float soft, float below) {
-    if (POWER == 1) return soft;
-    if (POWER == 2) return soft * soft;
-    if (POWER == 3) return soft * soft * soft;
-    if (POWER == 4) return (soft * soft) * (soft * soft);
-    return fast_exp2(below * kLog2e);
+    return TERMS == kSame ? soft : fast_exp2(below * kLog2e);
 }
-template <int POWER, bool HARD, int N>
+template <int TERMS, int N>
 __device__ __forceinline__ void add_terms(const f32x4 (&v)[N], float b, float cold, float& a, float& c) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
@@ -79,24 +76,21 @@ __device__ __forceinline__ void add_terms(const f32x4 (&v)[N], float b, float co
         for (int q = 0; q < 4; q++) {
             const float below = v[i][q] - b, t = fast_exp2(below * cold);
             a += t;
-            if (HARD) c += hard_term<POWER>(t, below);
+            if (TERMS != kSoft) c += hard_term<TERMS>(t, below);
         }
         __builtin_amdgcn_sched_barrier(0);   // one vector's temporaries at a time: the registers hold the row
     }
 }
 template <int N>
-__device__ __forceinline__ void stats_of(const f32x4 (&v)[N], float cold, bool hard, int power, RowStats& s) {
+__device__ __forceinline__ void stats_of(const f32x4 (&v)[N], float cold, int terms, RowStats& s) {
     float top = s.m;
 #pragma unroll
     for (int i = 0; i < N; i++) top = fmaxf(fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3])), top);
     const float b = RowStats::base(top);
     float a = s.st * fast_exp2((s.m - b) * cold), c = s.s1 * fast_exp2((s.m - b) * kLog2e);
-    if (!hard) add_terms<0, false>(v, b, cold, a, c);
-    else if (power == 1) add_terms<1, true>(v, b, cold, a, c);
-    else if (power == 2) add_terms<2, true>(v, b, cold, a, c);
-    else if (power == 3) add_terms<3, true>(v, b, cold, a, c);
-    else if (power == 4) add_terms<4, true>(v, b, cold, a, c);
-    else add_terms<0, true>(v, b, cold, a, c);
+    if (terms == kSoft) add_terms<kSoft>(v, b, cold, a, c);
+    else if (terms == kSame) add_terms<kSame>(v, b, cold, a, c);
+    else add_terms<kBoth>(v, b, cold, a, c);
     s.m = top; s.st = a; s.s1 = c;
 }
 
@@ -232,40 +226,36 @@ __global__ __launch_bounds__(1024) void distill_loss_kernel(const float* __restr
     }
 }
 
-struct GradRow { float cold, base, ct, c1; int power; };   // dz = ct exp2((z - base) cold) + c1 exp2((z - base) log2 e)
+struct GradRow { float cold, base, ct, c1; int terms; };   // dz = ct exp2((z - base) cold) + c1 exp2((z - base) log2 e)
 
 __device__ __forceinline__ GradRow grad_row(const DistillArgs& g, const Entries& e, const RowStats& s, float sum) {
     const float seed = g.seed ? g.seed[0] : 1.f, b = RowStats::base(s.m);
     const bool hard = g.w_hard != 0.f && e.index[g.topk] >= 0;
-    return {g.cold, b, sum != 0.f ? g.g_soft * seed / s.st : 0.f, hard ? g.g_hard * seed / s.s1 : 0.f, g.power};
+    return {g.cold, b, sum != 0.f ? g.g_soft * seed / s.st : 0.f, hard ? g.g_hard * seed / s.s1 : 0.f, g.terms};
 }
-// POWER as above; -1: without the softmax at 1
-template <int POWER>
+template <int TERMS>
 __device__ __forceinline__ float grad_term(const GradRow& r, float z) {
     const float below = z - r.base, t = fast_exp2(below * r.cold), d = r.ct * t;
-    return POWER < 0 ? d : fmaf(r.c1, hard_term<POWER>(t, below), d);
+    return TERMS == kSoft ? d : fmaf(r.c1, hard_term<TERMS>(t, below), d);
 }
-// calls f with the power as a constant: which it is holds for the whole launch, so the choice stands outside the loops
+// calls f with the terms as a constant: which they are holds for the whole launch, so the choice stands outside the loops
 template <typename F>
-__device__ __forceinline__ void with_power(bool hard, int power, F f) {
-    if (!hard) f(std::integral_constant<int, -1>{});
-    else if (power == 1) f(std::integral_constant<int, 1>{});
-    else if (power == 2) f(std::integral_constant<int, 2>{});
-    else if (power == 3) f(std::integral_constant<int, 3>{});
-    else if (power == 4) f(std::integral_constant<int, 4>{});
-    else f(std::integral_constant<int, 0>{});
+__device__ __forceinline__ void with_terms(int terms, F f) {
+    if (terms == kSoft) f(std::integral_constant<int, kSoft>{});
+    else if (terms == kSame) f(std::integral_constant<int, kSame>{});
+    else f(std::integral_constant<int, kBoth>{});
 }
-__device__ __forceinline__ float grad_at(const GradRow& r, bool hard, float z) {
+__device__ __forceinline__ float grad_at(const GradRow& r, float z) {
     float d = 0.f;
-    with_power(hard, r.power, [&](auto p) { d = grad_term<decltype(p)::value>(r, z); });
+    with_terms(r.terms, [&](auto t) { d = grad_term<decltype(t)::value>(r, z); });
     return d;
 }
 // the gradient is not read again here: its stores pass the caches by, which keep the logits (131072 logits: 476 us against 571)
-template <int POWER>
+template <int TERMS>
 __device__ __forceinline__ void grad_store(const GradRow& r, f32x4 v, float* __restrict__ dz, int i, int vecs) {
     f32x4 d;
 #pragma unroll
-    for (int q = 0; q < 4; q++) d[q] = grad_term<POWER>(r, v[q]);
+    for (int q = 0; q < 4; q++) d[q] = grad_term<TERMS>(r, v[q]);
     if (i < vecs) __builtin_nontemporal_store(d, reinterpret_cast<f32x4u*>(dz + 4 * (unsigned)i));
 }
 // the places of [begin, end) that the teacher or the label names, behind the dense stores
@@ -294,7 +284,7 @@ __device__ __forceinline__ void grad_entries(const DistillArgs& g, const Entries
                 w += o == g.topk ? hard : soft == 0.f ? 0.f : soft * fast_exp2((e.value[o] - top) * g.cold);
             }
         }
-        if (first) dz[i] = grad_at(r, g.w_hard != 0.f, e.logit[j]) - w;
+        if (first) dz[i] = grad_at(r, e.logit[j]) - w;
     }
 }
 
@@ -307,7 +297,6 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillArgs g) {
     const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
     const Span part(g.z + row * g.ldz, 0, g.vocab);
-    const bool hard = g.w_hard != 0.f;
     f32x4* held = reinterpret_cast<f32x4*>(lds);
     constexpr int GROUP = NV < 4 ? NV : 4, FIRST = (NV + LV) * THREADS;
     // the row's entries are asked for before its logits: their own logits are then on the way behind those
@@ -326,7 +315,7 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillArgs g) {
         f32x4 u[GROUP];
 #pragma unroll
         for (int q = 0; q < GROUP; q++) u[q] = v[i + q];
-        stats_of(u, g.cold, hard, g.power, s);
+        stats_of(u, g.cold, g.terms, s);
         __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (LV > 0) {
@@ -335,7 +324,7 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillArgs g) {
             f32x4 u[3];
 #pragma unroll
             for (int q = 0; q < 3; q++) u[q] = part.load<GRAD>(tid + (NV + i + q) * THREADS);
-            stats_of(u, g.cold, hard, g.power, s);
+            stats_of(u, g.cold, g.terms, s);
 #pragma unroll
             for (int q = 0; q < 3; q++) held[(i + q) * THREADS + tid] = u[q];
         }
@@ -344,7 +333,7 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillArgs g) {
         f32x4 u[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) u[i] = part.load(at + i * THREADS);
-        stats_of(u, g.cold, hard, g.power, s);
+        stats_of(u, g.cold, g.terms, s);
     }
     if (part.single(tid)) stats_of_one(rest, g.cold, s);
     s = block_stats<THREADS / 64>(s, g.cold, red);       // its barrier also publishes the entries
@@ -356,17 +345,17 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillArgs g) {
     const GradRow r = grad_row(g, e, s, sum);
     int again = tid;                                     // the stores' offsets are computed anew, not kept since the loads
     asm volatile("" : "+v"(again));
-    with_power(hard, g.power, [&](auto p) {
-        constexpr int POWER = decltype(p)::value;
+    with_terms(g.terms, [&](auto t) {
+        constexpr int TERMS = decltype(t)::value;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            grad_store<POWER>(r, v[i], dz, again + i * THREADS, part.vecs);
+            grad_store<TERMS>(r, v[i], dz, again + i * THREADS, part.vecs);
             __builtin_amdgcn_sched_barrier(0);           // four gradients in registers at a time, not all
         }
         if constexpr (LV > 0) {
 #pragma unroll
             for (int i = 0; i < LV; i++) {
-                grad_store<POWER>(r, held[i * THREADS + tid], dz, again + (NV + i) * THREADS, part.vecs);
+                grad_store<TERMS>(r, held[i * THREADS + tid], dz, again + (NV + i) * THREADS, part.vecs);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -375,10 +364,10 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillArgs g) {
 #pragma unroll
             for (int i = 0; i < 4; i++) u[i] = part.load(at + i * THREADS);
 #pragma unroll
-            for (int i = 0; i < 4; i++) grad_store<POWER>(r, u[i], dz, at + i * THREADS, part.vecs);
+            for (int i = 0; i < 4; i++) grad_store<TERMS>(r, u[i], dz, at + i * THREADS, part.vecs);
         }
     });
-    if (part.single(tid)) dz[part.place(tid)] = grad_at(r, hard, rest);
+    if (part.single(tid)) dz[part.place(tid)] = grad_at(r, rest);
     __syncthreads();
     grad_entries(g, e, r, top, sum, g.dz + row * g.ldd, 0, g.vocab, THREADS);
 }
@@ -402,7 +391,7 @@ __global__ __launch_bounds__(kSegThreads) void distill_segment_stats_kernel(Dist
         f32x4 u[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) u[i] = part.load(at + i * kSegThreads);
-        stats_of(u, g.cold, g.w_hard != 0.f, g.power, s);
+        stats_of(u, g.cold, g.terms, s);
     }
     if (part.single(threadIdx.x)) stats_of_one(part.rest(threadIdx.x), g.cold, s);
     s = block_stats<kSegThreads / 64>(s, g.cold, red);
@@ -452,16 +441,16 @@ __global__ __launch_bounds__(kSegThreads) void distill_segment_grad_kernel(Disti
     float* dz = g.dz + row * g.ldd;
     const GradRow r = grad_row(g, e, s, sum);
     const Span part(z, begin, end);
-    with_power(g.w_hard != 0.f, g.power, [&](auto p) {
+    with_terms(g.terms, [&](auto t) {
         for (int at = threadIdx.x; at < part.vecs; at += 4 * kSegThreads) {
             f32x4 u[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) u[i] = part.load(at + i * kSegThreads);
 #pragma unroll
-            for (int i = 0; i < 4; i++) grad_store<decltype(p)::value>(r, u[i], dz + begin + part.head, at + i * kSegThreads, part.vecs);
+            for (int i = 0; i < 4; i++) grad_store<decltype(t)::value>(r, u[i], dz + begin + part.head, at + i * kSegThreads, part.vecs);
         }
     });
-    if (part.single(threadIdx.x)) dz[begin + part.head + part.place(threadIdx.x)] = grad_at(r, g.w_hard != 0.f, part.rest(threadIdx.x));
+    if (part.single(threadIdx.x)) dz[begin + part.head + part.place(threadIdx.x)] = grad_at(r, part.rest(threadIdx.x));
     __syncthreads();
     grad_entries(g, e, r, top, sum, dz, begin, end, kSegThreads);
 }
@@ -487,9 +476,9 @@ static DistillArgs distill_args(const float* z, int64_t ldz, const float* teache
     g.rows = rows; g.vocab = (int)vocab; g.topk = (int)topk;
     g.inv_t = 1.f / temperature;
     g.cold = kLog2e / temperature;
-    g.power = temperature == 1.f ? 1 : temperature == 2.f ? 2 : temperature == 3.f ? 3 : temperature == 4.f ? 4 : 0;
     g.w_soft = alpha * temperature * temperature;
     g.w_hard = labels ? 1.f - alpha : 0.f;
+    g.terms = g.w_hard == 0.f ? kSoft : temperature == 1.f ? kSame : kBoth;
     g.g_soft = scale * alpha * temperature;
     g.g_hard = scale * (1.f - alpha);
     return g;

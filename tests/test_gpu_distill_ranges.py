@@ -96,3 +96,15 @@ def test_teacher_of_far_values(hip, rng):
     tol_row, tol_dz = bounds(z, spread, 0.5, 0.7, 1.0, 500)
     (row, _), _, dz, _ = run_distill(hip, z, teacher, index, lab, 0.5, 0.7, 1.0)
     assert (np.abs(row - want_row) <= tol_row + 4 * oc.U * np.abs(want_row)).all() and (np.abs(dz - want_dz) <= tol_dz).all()
+
+
+@pytest.mark.parametrize("rows,vocab", SHAPES)
+def test_the_temperature_leaves_the_hard_part_alone(hip, rng, rows, vocab):
+    """Without weight on the teacher the loss is a cross entropy at temperature 1, whatever the temperature: the same bits."""
+    case = distill_case(rng, rows, vocab, 3)
+    want = run_distill(hip, *case, 1.0, 0.0, 0.5)
+    for temperature in (2.0, 2.5, 3.0, 4.0):
+        got = run_distill(hip, *case, temperature, 0.0, 0.5)
+        for (row, loss), (row1, loss1) in zip(got[:2], want[:2]):
+            assert np.array_equal(row, row1) and loss == loss1
+        assert np.array_equal(got[2], want[2]) and np.array_equal(got[3], want[3]), temperature
