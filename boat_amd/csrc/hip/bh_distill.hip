@@ -473,7 +473,8 @@ static DistillArgs distill_args(const float* z, int64_t ldz, const float* teache
                                 int64_t vocab, int64_t topk, float temperature, float alpha, float scale) {
     DistillArgs g = {};
     g.z = z; g.ldz = ldz; g.teacher = teacher; g.index = index; g.labels = labels;
-    g.rows = rows; g.vocab = (int)vocab; g.topk = (int)topk;
+    // a teacher without weight is not looked at: a divergence that is infinite would make 0 times infinity of it
+    g.rows = rows; g.vocab = (int)vocab; g.topk = alpha == 0.f ? 0 : (int)topk;
     g.inv_t = 1.f / temperature;
     g.cold = kLog2e / temperature;
     g.w_soft = alpha * temperature * temperature;

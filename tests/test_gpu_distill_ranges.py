@@ -108,3 +108,20 @@ def test_the_temperature_leaves_the_hard_part_alone(hip, rng, rows, vocab):
         for (row, loss), (row1, loss1) in zip(got[:2], want[:2]):
             assert np.array_equal(row, row1) and loss == loss1
         assert np.array_equal(got[2], want[2]) and np.array_equal(got[3], want[3]), temperature
+
+
+@pytest.mark.parametrize("rows,vocab", SHAPES)
+def test_a_teacher_without_weight_is_not_looked_at(hip, rng, rows, vocab):
+    """alpha = 0: masked student logits under the teacher's entries, or a teacher of NaN, leave the cross entropy as it is."""
+    z, teacher, index, lab = distill_case(rng, rows, vocab, 6)
+    for r in range(rows):
+        for i in index[r]:
+            if 0 <= i < vocab and i != lab[r]:
+                z[r, i] = -np.inf
+    none = np.zeros((rows, 0), np.float32), np.zeros((rows, 0), np.int32)
+    want = run_distill(hip, z, *none, lab, 2.0, 0.0, 0.5)
+    assert np.isfinite(want[0][0]).all() and np.isfinite(want[2]).all()
+    for t in (teacher, np.full_like(teacher, np.nan), np.full_like(teacher, np.inf)):
+        got = run_distill(hip, z, t, index, lab, 2.0, 0.0, 0.5)
+        assert np.array_equal(got[0][0], want[0][0]) and got[0][1] == want[0][1] and np.array_equal(got[1][0], want[1][0])
+        assert np.array_equal(got[2], want[2]) and np.array_equal(got[3], want[3])
