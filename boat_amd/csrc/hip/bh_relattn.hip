@@ -338,8 +338,9 @@ __device__ __forceinline__ void store_forward(const RelArgs& g, const f32x16 (&o
         if (lane < 32) { g.part_ml[2 * at] = m; g.part_ml[2 * at + 1] = l; }
     } else {
         dst = g.out + bh / g.heads * g.os[0] + bh % g.heads * g.os[1] + qi * g.os[2];
-        f = m == -INFINITY ? 0.f : 1.f / l;                                   // a row that sees nothing is zero
-        if (lane < 32) g.lse[row] = m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+        // a row that sees nothing has the sum 0 and is zero; one whose scores are NaN has no maximum either, but the sum NaN
+        f = l == 0.f ? 0.f : 1.f / l;
+        if (lane < 32) g.lse[row] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
     }
 #pragma unroll
     for (int b = 0; b < DP / 32; b++)
@@ -618,7 +619,7 @@ __global__ __launch_bounds__(256) void relattn_join_kernel(RelArgs g) {
     for (int x = 1; x < 16; x *= 2) sum += __shfl_xor(sum, x, 64);
     const int64_t bh = row / g.sq, qi = row - bh * g.sq, bt = bh / g.heads, h = bh - bt * g.heads;
     float* dst = g.out + bt * g.os[0] + h * g.os[1] + qi * g.os[2];
-    const float f = top == -INFINITY ? 0.f : 1.f / sum;
+    const float f = sum == 0.f ? 0.f : 1.f / sum;                             // as in store_forward
     const bool vec = g.d % 4 == 0;
     for (int c0 = 0; c0 < g.d; c0 += 64) {
         const int c = c0 + 4 * lane, n = min(4, g.d - c), at = min(c, g.d - 1) & (vec ? ~3 : ~0);
@@ -653,7 +654,7 @@ __global__ __launch_bounds__(256) void relattn_join_kernel(RelArgs g) {
                     if (j < n) dst[c + j] = a[j];
         }
     }
-    if (mine < rows && lane == 0) g.lse[row] = top == -INFINITY ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (mine < rows && lane == 0) g.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------------------------------- backward
