@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void relattn_split_kernel(SplitJobs a) {
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] = x[r][8 * c + e];
             u32x4 p[kPlanes];
-            split_eight(y, p);
+            split_eight<true>(y, p);
 #pragma unroll
             for (int q = 0; q < kPlanes; q++) *reinterpret_cast<u32x4*>(j.row + at + q * Block<DP>::PLANE + i * 16) = p[q];
         }
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256) void relattn_split_kernel(SplitJobs a) {
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] = x[r0 + (e < 4 ? e : e + 4)][c];
             u32x4 p[kPlanes];
-            split_eight(y, p);
+            split_eight<true>(y, p);
 #pragma unroll
             for (int q = 0; q < kPlanes; q++) *reinterpret_cast<u32x4*>(j.col + at + q * Block<DP>::PLANE + i * 16) = p[q];
         }
@@ -427,7 +427,7 @@ __global__ __launch_bounds__(kThreads, 2) void relattn_forward_kernel(RelArgs g)
     for (int s = 0; s < KD; s++) {
         float x[8];
         row_eight(q + min((int64_t)qi, g.sq - 1) * g.qs[2], true, 16 * s + 8 * (lane >> 5), g.d, g.vec_q, x);
-        split_eight(x, qf[s]);
+        split_eight<true>(x, qf[s]);
     }
     f32x16 o[ND];
 #pragma unroll
@@ -500,7 +500,7 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 96 ? 2 : 1) void relattn_rows
     for (int s = 0; s < KD; s++) {
         float x[8];
         row_eight(g.q + bt * g.qs[0] + h * g.qs[1] + qi * g.qs[2], true, 16 * s + 8 * (lane >> 5), g.d, g.vec_q, x);
-        split_eight(x, qf[s]);
+        split_eight<true>(x, qf[s]);
     }
     f32x16 o[ND];
 #pragma unroll
@@ -526,7 +526,7 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 96 ? 2 : 1) void relattn_rows
 #pragma unroll
         for (int t = 0; t < KD; t++) {
             u32x4 a[kPlanes];
-            split_eight(x[t], a);
+            split_eight<true>(x[t], a);
             s[0] = mfma_split(a, qf[t], s[0]);
         }
         const int rel0 = k0 - pos;                                            // the block's first key as this row sees it
@@ -555,7 +555,7 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 96 ? 2 : 1) void relattn_rows
 #pragma unroll
             for (int b = 0; b < ND; b++) {
                 u32x4 a[kPlanes];
-                split_eight(y[t][b], a);
+                split_eight<true>(y[t][b], a);
                 o[b] = mfma_split(a, p, o[b]);
             }
         }
@@ -721,11 +721,11 @@ __device__ __forceinline__ void query_tile(const RelArgs& g, int id, int part) {
         row_eight(q + qrow * g.qs[2], live, 16 * s + 8 * (lane >> 5), g.d, g.vec_q, x);
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] *= sign;
-        split_eight(x, qf[s]);
+        split_eight<true>(x, qf[s]);
         row_eight(dout + qrow * g.os[2], live, 16 * s + 8 * (lane >> 5), g.d, g.vec_o, x);
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] *= sign;
-        split_eight(x, gf[s]);
+        split_eight<true>(x, gf[s]);
     }
     const int64_t row = (int64_t)bh * g.sq + qrow;
     const float lse = lse_log2(g.lse_in[row]), delta = g.delta[row];
@@ -868,9 +868,9 @@ __device__ __forceinline__ void key_tile(const RelArgs& g, int id, int part) {
     for (int s = 0; s < KD; s++) {
         float x[8];
         row_eight(k + min((int64_t)ki, g.sk - 1) * g.ks[2], live, 16 * s + 8 * (lane >> 5), g.d, g.vec_k, x);
-        split_eight(x, kf[s]);
+        split_eight<true>(x, kf[s]);
         row_eight(v + min((int64_t)ki, g.sk - 1) * g.vs[2], live, 16 * s + 8 * (lane >> 5), g.d, g.vec_v, x);
-        split_eight(x, vf[s]);
+        split_eight<true>(x, vf[s]);
     }
     f32x16 dk[ND], dv[ND];
 #pragma unroll

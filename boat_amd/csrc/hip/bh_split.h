@@ -8,10 +8,12 @@
 // 2 * 2^-9 * 2^-18 + 2^-36 < 2^-25 of |a*b|: half of what rounding the product itself to fp32 may cost (2^-24).  So the sums
 // are fp32 sums, and six v_mfma_f32_32x32x16_bf16 take 192 cycles of a SIMD for what takes v_mfma_f32_32x32x2_f32 512.
 //
-// Where the split does not hold it shows: an infinity (or a value that rounds to one as a bf16) leaves NaN in its remainders,
-// and any sum it enters ends as NaN.  The kernels look for sums that are not finite and recompute those in plain fp32
-// arithmetic from memory, so infinities and NaN come out as fp32 arithmetic gives them.  The parts of values below 2^-110
-// become subnormal; the matrix cores keep subnormals.
+// Where the split does not hold it shows: an infinity leaves NaN in its remainders, and any sum it enters ends as NaN.  So does a
+// finite value past the largest bf16 (3.3895e38; from 3.396e38 on the first part would be an infinity) unless the first part is
+// kept to that bf16 (WIDE), which takes one instruction more a value; the remainder is then still exact.  What the kernels make of it: the dense
+// product looks for sums that are not finite and makes those again in plain fp32 arithmetic from memory, so infinities and NaN
+// come out as fp32 arithmetic gives them; attention splits its operands WIDE, and an infinity in them ends as NaN.  The parts of
+// values below 2^-110 become subnormal; the matrix cores keep subnormals.
 #pragma once
 
 #include "bh_common.h"
@@ -28,8 +30,11 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kPlanes = 3;   // h, m, l
 
 // two floats to their three packed bf16 pairs
+template <bool WIDE = false>
 __device__ __forceinline__ void split_pair(float x, float y, unsigned& h, unsigned& m, unsigned& l) {
-    h = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){x, y}, bf16x2));
+    constexpr float kMost = 3.38953139e38f;      // the largest bf16
+    const f32x2 first = WIDE ? (f32x2){__builtin_amdgcn_fmed3f(x, -kMost, kMost), __builtin_amdgcn_fmed3f(y, -kMost, kMost)} : (f32x2){x, y};
+    h = __builtin_bit_cast(unsigned, __builtin_convertvector(first, bf16x2));
     const float rx = x - __uint_as_float(h << 16), ry = y - __uint_as_float(h & 0xffff0000u);
     m = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){rx, ry}, bf16x2));
     const float sx = rx - __uint_as_float(m << 16), sy = ry - __uint_as_float(m & 0xffff0000u);
@@ -37,11 +42,12 @@ __device__ __forceinline__ void split_pair(float x, float y, unsigned& h, unsign
 }
 
 // eight floats, consecutive in the contraction index, to a lane's fragment in each plane
+template <bool WIDE = false>
 __device__ __forceinline__ void split_eight(const float (&x)[8], u32x4 (&p)[kPlanes]) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         unsigned h, m, l;
-        split_pair(x[2 * i], x[2 * i + 1], h, m, l);
+        split_pair<WIDE>(x[2 * i], x[2 * i + 1], h, m, l);
         p[0][i] = h; p[1][i] = m; p[2][i] = l;
     }
 }

@@ -325,7 +325,11 @@ int bh_sdpa_backward_cached(const float* q, const float* k, const float* v, cons
  * kv_len [batch] (or NULL) holds the number of valid keys of each sequence, values outside [0, sk] counting as the nearer
  * end: what lies behind them is not read.  causal: a query sees keys with r <= 0 only.  What a
  * key holds that only this mask or its bucket hides has to be finite: its weight is 0, and 0 times infinity is not.  A query that
- * sees no key has out = 0, lse = -inf and no gradient.  lse [batch, heads, sq], dense. */
+ * sees no key has out = 0, lse = -inf and no gradient.  lse [batch, heads, sq], dense.
+ * q, k, v and d_out may hold any finite value as long as the sums stay in range before their division by the sum of weights or
+ * their scaling; an infinity that a query sees ends as NaN (not as an infinity), a NaN as NaN.  The backward pass makes the
+ * weights again as exp(x - lse): they are off by 2^-23 |lse| relative, so a table value that is meant as a mask is -1e30 or less,
+ * not a number like -1e9 that every key of some query may have. */
 typedef struct bh_relbias_attention {
     int64_t batch, heads, kv_heads, sq, sk, d;
     int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
