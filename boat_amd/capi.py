@@ -43,7 +43,7 @@ class AttentionConfig(C.Structure):  # include/boat/layers/attention.h:21-30
 class RelativeAttentionConfig(C.Structure):
     """boat_hip_relative_attention_config_t."""
     _fields_ = [("num_buckets", C.c_int), ("max_distance", C.c_int), ("bidirectional", C.c_bool), ("causal", C.c_bool),
-                ("query_offset", C.c_int64), ("scale", C.c_float)]
+                ("query_offset", C.c_int64), ("scale", C.c_float), ("queries_at_end", C.c_bool)]
 
 
 class LayerNormConfig(C.Structure):  # include/boat/layers/norm.h:21-26

@@ -44,6 +44,7 @@ struct RelArgs {
     int64_t qs[3], ks[3], vs[3], os[3];    // strides of batch, head, row
     int batch, heads, kv_heads, group, d;
     int64_t sq, sk, offset;
+    int at_end;                            // the offset counts from a sequence's own last sq keys
     int causal;
     float scale;
     bool vec_q, vec_k, vec_v, vec_o;
@@ -59,6 +60,12 @@ struct RelArgs {
     float *part_k, *part_v;                // shared key heads or split queries: [split][batch*heads][sk][d]
     Buckets b;
 };
+
+// valid keys of a sequence, and the position of its first query
+__device__ __forceinline__ int length_of(const RelArgs& g, int bt) {
+    return g.kv_len ? __builtin_amdgcn_readfirstlane(min(max(g.kv_len[bt], 0), (int)g.sk)) : (int)g.sk;
+}
+__device__ __forceinline__ int64_t offset_of(const RelArgs& g, int len) { return g.at_end ? g.offset + len - g.sq : g.offset; }
 
 // ---- the bias as a workgroup sees it.  Where the borders span no more than kLine relative positions LDS holds the bias (times
 // log2 e) and the bucket of each of them, worked out once; else the borders and the head's table column, and every wavefront
@@ -414,11 +421,12 @@ __global__ __launch_bounds__(kThreads, 2) void relattn_forward_kernel(RelArgs g)
 
     const int q0 = tile * kQueryTile, qw = q0 + 32 * wave;                    // this wavefront's queries: qw + 0..31
     const int qi = qw + (lane & 31);
-    const int len = g.kv_len ? min(max(g.kv_len[bt], 0), (int)g.sk) : (int)g.sk;
+    const int len = length_of(g, bt);
+    const int64_t offset = offset_of(g, len);
     int seen = len;                                                           // keys that some query of the workgroup sees
-    if (g.causal) seen = (int)min((int64_t)seen, max((int64_t)0, min((int64_t)q0 + kQueryTile, g.sq) + g.offset));
+    if (g.causal) seen = (int)min((int64_t)seen, max((int64_t)0, min((int64_t)q0 + kQueryTile, g.sq) + offset));
     const int kb = (int)min((int64_t)seen, blockIdx.y * g.keys_per_split), ke = (int)min((int64_t)seen, kb + g.keys_per_split);
-    const int rel_q = (int)(qw + g.offset);                                   // position of the wavefront's first query
+    const int rel_q = (int)(qw + offset);                                   // position of the wavefront's first query
     if (kb < ke) {
         copy_to_lds<2 * NB * DP * 96 / 1024, kWaves>(kp + (int64_t)(kb / 32) * Block<DP>::BYTES, smem, wave, lane);
     }
@@ -490,11 +498,12 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 96 ? 2 : 1) void relattn_rows
     const float* v = g.v + bt * g.vs[0] + hk * g.vs[1];
     for (int i = tid; i <= g.b.far; i += 64 * kRowWaves) border[i] = g.b.border[i];
     __syncthreads();
-    const int len = g.kv_len ? min(max(g.kv_len[bt], 0), (int)g.sk) : (int)g.sk;
-    const int seen = g.causal ? (int)max((int64_t)0, min((int64_t)len, g.sq + g.offset)) : len;
+    const int len = length_of(g, bt);
+    const int64_t offset = offset_of(g, len);
+    const int seen = g.causal ? (int)max((int64_t)0, min((int64_t)len, g.sq + offset)) : len;
     const int unit = 32 * kRowWaves, per = ((seen + unit - 1) / unit + g.splits - 1) / g.splits * unit;
     const int kb = (int)min((int64_t)seen, (int64_t)blockIdx.y * per), ke = (int)min((int64_t)seen, (int64_t)kb + per);
-    const int pos = (int)(qi + g.offset);
+    const int pos = (int)(qi + offset);
     u32x4 qf[KD][kPlanes];
 #pragma unroll
     for (int s = 0; s < KD; s++) {
@@ -697,12 +706,13 @@ __device__ __forceinline__ void query_tile(const RelArgs& g, int id, int part) {
 
     const int q0 = tile * kQueryTile, qw = q0 + 32 * wave, qi = qw + (lane & 31);
     const bool live = qi < g.sq;
-    const int len = g.kv_len ? min(max(g.kv_len[bt], 0), (int)g.sk) : (int)g.sk;
+    const int len = length_of(g, bt);
+    const int64_t offset = offset_of(g, len);
     int ke = len;
-    if (g.causal) ke = (int)min((int64_t)ke, max((int64_t)0, min((int64_t)q0 + kQueryTile, g.sq) + g.offset));
+    if (g.causal) ke = (int)min((int64_t)ke, max((int64_t)0, min((int64_t)q0 + kQueryTile, g.sq) + offset));
     const int kb = (int)(part * g.keys_per_split);
     ke = (int)min((int64_t)ke, kb + g.keys_per_split);
-    const int rel_q = (int)(qw + g.offset);
+    const int rel_q = (int)(qw + offset);
     const auto fetch_rows = [&](int k0) {
         const int64_t at = plane0 + (int64_t)(k0 / 32) * Block<DP>::BYTES;
         copy_to_lds<KB, kWaves>(g.k_row + at, smem, wave, lane);
@@ -861,7 +871,8 @@ __device__ __forceinline__ void key_tile(const RelArgs& g, int id, int part) {
     const float* k = g.k + bt * g.ks[0] + hk * g.ks[1];
     const float* v = g.v + bt * g.vs[0] + hk * g.vs[1];
     const int kw = tile * 128 + 32 * wave, ki = kw + (lane & 31), sq = (int)g.sq;
-    const int len = g.kv_len ? min(max(g.kv_len[bt], 0), (int)g.sk) : (int)g.sk;
+    const int len = length_of(g, bt);
+    const int64_t offset = offset_of(g, len);
     const bool live = ki < len;
     u32x4 kf[KD][kPlanes], vf[KD][kPlanes];
 #pragma unroll
@@ -877,7 +888,7 @@ __device__ __forceinline__ void key_tile(const RelArgs& g, int id, int part) {
     for (int b = 0; b < ND; b++) { dk[b] = zero16(); dv[b] = zero16(); }
     const float c = g.scale * kLog2e;
     int qb = 0;                                                               // causal: the first query that sees a key of the workgroup
-    if (g.causal) qb = (int)(min((int64_t)sq, max((int64_t)0, (int64_t)tile * 128 - g.offset)) / ROWS * ROWS);
+    if (g.causal) qb = (int)(min((int64_t)sq, max((int64_t)0, (int64_t)tile * 128 - offset)) / ROWS * ROWS);
     const int qe = min(sq, (part + 1) * g.queries_per_split);
     qb = max(qb, part * g.queries_per_split);
     if (tile * 128 >= len) qb = sq;                                           // only padding here
@@ -909,7 +920,7 @@ __device__ __forceinline__ void key_tile(const RelArgs& g, int id, int part) {
             fetch(g.q_col, g.g_col, r0, L::QT);
             if (r0 > qb) fetch_stat(r0 - ROWS, turn ^ 1);
             const float* stat = reinterpret_cast<const float*>(smem + L::STAT) + 64 * turn;
-            const bool mine = kw < len && !(g.causal && kw > min(r0 + ROWS, sq) - 1 + g.offset);
+            const bool mine = kw < len && !(g.causal && kw > min(r0 + ROWS, sq) - 1 + offset);
             f32x16 s, dp;
             if (mine) {
                 s = zero16();
@@ -924,7 +935,7 @@ __device__ __forceinline__ void key_tile(const RelArgs& g, int id, int part) {
             if (r0 > qb) fetch(g.q_row, g.g_row, r0 - ROWS, 0);
             if (mine) {
             // block [32 queries as rows][32 keys as columns]
-            const int rel0 = (int)(kw - r0 - g.offset);
+            const int rel0 = (int)(kw - r0 - offset);
             const int constant = constant_bucket(g.b, rel0 - 31, rel0 + 31);
             const f32x4* ls = reinterpret_cast<const f32x4*>(stat + 4 * (lane >> 5));   // lse of rows 8g + 4 half + 0..3
             if (constant >= 0) {
@@ -1132,7 +1143,7 @@ static int relattn_args(const char* fn, const bh_relbias_attention_t* p, RelArgs
     if (p->batch < 0 || p->heads < 0 || p->kv_heads < 0 || p->sq < 0 || p->sk < 0) return set_error(BH_EINVAL, "%s: negative dimension", fn);
     if (p->d < 1 || p->d > 128) return set_error(BH_EINVAL, "%s: the head size is 1 to 128", fn);
     if (p->heads > 0 && (p->kv_heads < 1 || p->heads % p->kv_heads)) return set_error(BH_EINVAL, "%s: heads is a multiple of kv_heads", fn);
-    const int64_t most = (int64_t)1 << 28;                // sums and differences of them stay within 32 bits
+    const int64_t most = (int64_t)1 << 28;                // sums and differences of them (up to five) stay within 32 bits
     if (p->sq > most || p->sk > most || p->query_offset > most || p->query_offset < -most)
         return set_error(BH_EINVAL, "%s: sequences and offset are at most 2^28", fn);
     if (p->batch > 0x7fffffff || p->heads > 0x7fffffff || p->batch * p->heads > 0x7fffffff / 2) return set_error(BH_EINVAL, "%s: too many heads", fn);
@@ -1146,7 +1157,7 @@ static int relattn_args(const char* fn, const bh_relbias_attention_t* p, RelArgs
     if (!(fabsf(p->scale) < INFINITY)) return set_error(BH_EINVAL, "%s: the scale is a number", fn);
     g.batch = (int)p->batch; g.heads = (int)p->heads; g.kv_heads = (int)p->kv_heads;
     g.group = p->heads ? (int)(p->heads / p->kv_heads) : 1;
-    g.d = (int)p->d; g.sq = p->sq; g.sk = p->sk; g.offset = p->query_offset; g.causal = p->causal ? 1 : 0; g.scale = p->scale;
+    g.d = (int)p->d; g.sq = p->sq; g.sk = p->sk; g.offset = p->query_offset; g.causal = p->causal ? 1 : 0; g.at_end = p->queries_at_end ? 1 : 0; g.scale = p->scale;
     for (int i = 0; i < 3; i++) { g.qs[i] = p->q_stride[i]; g.ks[i] = p->k_stride[i]; g.vs[i] = p->v_stride[i]; g.os[i] = p->o_stride[i]; }
     g.buckets = p->num_buckets;
     g.q_tiles = (int)ceil_div(p->sq, kQueryTile);
@@ -1229,10 +1240,11 @@ static int parts_for(int64_t wgs, int64_t longest, double mean, int each, int st
 // the pairs of query and key that a causal mask leaves
 static double seen_pairs(const RelArgs& g) {
     if (!g.causal) return (double)g.sq * (double)g.sk;
+    const int64_t offset = g.at_end ? g.sk - g.sq + g.offset : g.offset;       // as in a sequence of full length
     // query i sees min(max(i + 1 + offset, 0), sk) keys: none below lo, all from hi on
-    const int64_t lo = -g.offset < 0 ? 0 : -g.offset < g.sq ? -g.offset : g.sq, full = g.sk - 1 - g.offset;
+    const int64_t lo = -offset < 0 ? 0 : -offset < g.sq ? -offset : g.sq, full = g.sk - 1 - offset;
     const int64_t hi = full < lo ? lo : full < g.sq ? full : g.sq;
-    return ((double)(lo + 1 + g.offset) + (double)(hi + g.offset)) * 0.5 * (double)(hi - lo) + (double)(g.sq - hi) * (double)g.sk;
+    return ((double)(lo + 1 + offset) + (double)(hi + offset)) * 0.5 * (double)(hi - lo) + (double)(g.sq - hi) * (double)g.sk;
 }
 
 template <int DP>

@@ -102,7 +102,7 @@ static bool relative_plan(const boat_hip_relative_attention_config_t* c, const b
         .q_stride = {q->shape[1] * h * d, d, h * d}, .k_stride = {k->shape[1] * g * d, d, g * d},
         .v_stride = {k->shape[1] * g * d, d, g * d}, .o_stride = {q->shape[1] * h * d, d, h * d},
         .query_offset = c->query_offset, .num_buckets = c->num_buckets, .max_distance = c->max_distance,
-        .bidirectional = c->bidirectional, .causal = c->causal, .scale = c->scale};
+        .bidirectional = c->bidirectional, .causal = c->causal, .scale = c->scale, .queries_at_end = c->queries_at_end};
     *p = plan;
     return true;
 }

@@ -27,7 +27,7 @@ class RelbiasAttention(C.Structure):
     """bh_relbias_attention_t."""
     _fields_ = [(n, L) for n in ("batch", "heads", "kv_heads", "sq", "sk", "d")] + [
         (n, L * 3) for n in ("q_stride", "k_stride", "v_stride", "o_stride")] + [("query_offset", L)] + [
-        (n, C.c_int32) for n in ("num_buckets", "max_distance", "bidirectional", "causal")] + [("scale", F)]
+        (n, C.c_int32) for n in ("num_buckets", "max_distance", "bidirectional", "causal")] + [("scale", F), ("queries_at_end", C.c_int32)]
 
 
 _SIGS = {

@@ -514,13 +514,15 @@ BOAT_API boat_variable_t* boat_hip_var_dense_act(const boat_variable_t* input, b
  * (neighbouring heads share a key head); table [num_buckets, heads]; lengths: NULL or INT32 [batch], the number of valid
  * keys of each sequence.  head_size at most 128.  So the [batch*seq, heads*head_size] output of a dense layer is reshaped,
  * never transposed.  Returns the shape of query; *lse (may be NULL) receives the [batch, heads, seq_q] row log-sum-exp.
- * query_offset: position of the first query counted from the first key (seq_k - seq_q for the last tokens of a sequence). */
+ * query_offset: position of the first query counted from the first key (seq_k - seq_q for the last tokens of sequences of seq_k
+ * keys); with queries_at_end counted from lengths[b] - seq_q instead, so that 0 stands for the last tokens of each sequence. */
 typedef struct {
     int num_buckets, max_distance;
     bool bidirectional;          /* half of the buckets for keys behind the query, half for keys ahead */
     bool causal;
     int64_t query_offset;
     float scale;
+    bool queries_at_end;
 } boat_hip_relative_attention_config_t;
 BOAT_API boat_tensor_t* boat_hip_relative_attention(const boat_hip_relative_attention_config_t* config, const boat_tensor_t* query,
                                                     const boat_tensor_t* key, const boat_tensor_t* value,

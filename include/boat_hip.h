@@ -333,9 +333,11 @@ int bh_sdpa_backward_cached(const float* q, const float* k, const float* v, cons
 typedef struct bh_relbias_attention {
     int64_t batch, heads, kv_heads, sq, sk, d;
     int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
-    int64_t query_offset;      /* position of query 0 counted from key 0: sk - sq where the queries are the last tokens */
+    int64_t query_offset;      /* position of query 0 counted from key 0: sk - sq for the last tokens of sequences of sk keys */
     int32_t num_buckets, max_distance, bidirectional, causal;
     float scale;
+    int32_t queries_at_end;    /* nonzero: query_offset counts from kv_len[b] - sq, so that 0 stands for the last sq tokens of
+                                * each sequence of a padded batch (a decoder's new tokens) */
 } bh_relbias_attention_t;
 /* the bucket of one relative position (host arithmetic), or BH_EINVAL */
 int bh_relative_position_bucket(int64_t relative, int num_buckets, int max_distance, int bidirectional);
