@@ -30,8 +30,10 @@ struct EpiArgs {
     float* colsum; int colsum_add;           // small tiles, both operands along rows: [n] (+)= column sums of B, or NULL
 };
 
-// erf as GELU needs it, to an absolute 9e-8 (1 + erf rounds to 6e-8 anyway), without a branch: 1 - erf(t) = 2^(-t P(t)), P the
-// polynomial of degree 8 whose largest error in erf over [0, 4] is least (by linear programming); from 4 on erf is 1 in fp32.
+// erf as GELU needs it, without a branch: 1 - erf(t) = 2^(-t P(t)), P the polynomial of degree 8 whose largest error in erf over
+// [0, 4] is least (by linear programming); from 4 on erf is 1 in fp32.  Evaluated in fp32 it is off by at most 9.1e-8, and the
+// hardware exponential adds up to one step of [1/2, 1): 1.5e-7 absolute, where 1 + erf rounds to 6e-8.  The GELU of a dense sweep
+// of [-6, 6] is off by at most 1.13e-7 |z| (1.22e-7 with erff), next to zero by 7.7e-8 |z| (6.2e-8).
 // 8192 x 4096 over 1024 with GELU and z kept 335 us, 349 with erff, 330 without an activation.
 __device__ __forceinline__ float erf_absolute(float x) {
     const float t = fminf(fabsf(x), 4.f);

@@ -281,6 +281,7 @@ int bh_dense_backward_into(const float* x, const float* w, const float* dy,
  * BH_ACT_* or BH_ACT_NONE.  bias, saved and residual may be NULL.  saved [M,N] (leading dimension lds) receives what
  * bh_activation_backward wants: z, or act(z) for BH_ACT_SIGMOID and BH_ACT_TANH.  residual [M,N] (ldr) may be C itself
  * (C += act(z)); otherwise no output may overlap an operand.  K == 0: z = bias.
+ * GELU is off by less than 2e-7 |z| and may differ in its last bits from bh_activation_forward's.
  * fp32 sums on the bf16 matrix cores (each operand as the exact sum of three bf16, six partial products: the error of an
  * fp32 product and sum); infinities and NaN come out as fp32 arithmetic gives them. */
 int bh_gemm_epilogue(int trans_a, int trans_b, int64_t m, int64_t n, int64_t k, const float* a, int64_t lda, const float* b,
