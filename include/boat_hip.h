@@ -283,7 +283,8 @@ int bh_dense_backward_into(const float* x, const float* w, const float* dy,
  * (C += act(z)); otherwise no output may overlap an operand.  K == 0: z = bias.
  * GELU is off by less than 2e-7 |z| and may differ in its last bits from bh_activation_forward's.
  * fp32 sums on the bf16 matrix cores (each operand as the exact sum of three bf16, six partial products: the error of an
- * fp32 product and sum); infinities and NaN come out as fp32 arithmetic gives them. */
+ * fp32 product and sum); infinities and NaN come out as fp32 arithmetic gives them.  An infinite sum is made again term by term:
+ * a matrix full of them takes up to 200 times as long as a finite one, a matrix of NaN about twice as long. */
 int bh_gemm_epilogue(int trans_a, int trans_b, int64_t m, int64_t n, int64_t k, const float* a, int64_t lda, const float* b,
                      int64_t ldb, float* c, int64_t ldc, const float* bias, int act, float* saved, int64_t lds,
                      const float* residual, int64_t ldr);
