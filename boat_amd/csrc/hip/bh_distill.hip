@@ -372,7 +372,7 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(DistillArgs g) {
     grad_entries(g, e, r, top, sum, g.dz + row * g.ldd, 0, g.vocab, THREADS);
 }
 
-// ---- rows cut into segments (37 rows of 128001 logits: 6.6 us for the statistics and 10 us for loss and gradient, which find the
+// ---- rows cut into segments (37 rows of 128001 logits: 7 us for the statistics and 10 us for loss and gradient, which find the
 // 38 MB in the memory-side cache; with a workgroup per row 37 of 256 compute units would work)
 constexpr int kSegThreads = 256;
 __global__ __launch_bounds__(kSegThreads) void distill_segment_stats_kernel(DistillArgs g) {
@@ -416,7 +416,8 @@ __device__ __forceinline__ RowStats joined_stats(const DistillArgs& g, int64_t r
     return s;
 }
 
-// the gradient of a row's segment from statistics: the segments' (with the row's loss), or those a forward call kept
+// the gradient of a row's segment from statistics: the segments' (with the row's loss), or those a forward call kept (8192 x 50001:
+// 697 us, 4.7 TB/s, behind a forward pass of 281 us; both in one read the logits once, 673 us)
 template <bool JOIN, bool GRAD>
 __global__ __launch_bounds__(kSegThreads) void distill_segment_grad_kernel(DistillArgs g) {
     extern __shared__ float lds[];

@@ -271,8 +271,9 @@ struct TileLds {
     static constexpr int BYTES = 2 * STAGE > EPI ? 2 * STAGE : EPI;
 };
 
-// Bound by the matrix cores: 8192 x 4096 over 1024 with GELU and z kept 335 us (205 TFLOP/s; 268 MB of stores that little runs
-// beside), its dX 307 us (224), its dW 319 us (215), 8192 x 1024 over 1024 with a residual 110 us (156).
+// Bound by the matrix cores, which are busy for 60 to 76 % of the cycles, at a clock that falls to 1.9 GHz: 8192 x 4096 over 1024
+// with GELU and z kept 335 us (205 TFLOP/s; 268 MB of stores that little runs beside), its dX 307 us (224), its dW 319 us (215),
+// 8192 x 1024 over 1024 with a residual 110 us (156; 49 % of the cycles).
 // VEC: the operands whose contraction index is the fast one can be read 16 bytes at a time
 template <typename Cfg, bool A_KC, bool B_KC, bool VEC>
 __global__ __launch_bounds__(Cfg::NT, Cfg::WGS) void epilogue_tile_kernel(EpiArgs g, bool vec_c) {
@@ -401,8 +402,9 @@ __global__ __launch_bounds__(256) void epilogue_fold_kernel(EpiArgs g) {
 // ---------------------------------------------------------------------------------------------------- small products
 // Outputs that fill few tiles: a workgroup owns a 32 x 32 tile and its wavefronts cut the contraction, each splitting its
 // fragments straight from memory in registers; their sums meet in LDS.  No barrier and no LDS in the loop, so a wavefront
-// keeps several steps' loads in flight, which is what such a product waits for: 1 x 4096 over 1024 (16.8 MB of weights) 7.7 us,
-// 777 x 513 over 784 13.5 us.  (Loads a step further ahead, with the registers for it taken from the addresses, were slower: 14.5 us.)
+// keeps several steps' loads in flight, which is what such a product waits for: 1 x 4096 over 1024 (16.8 MB of weights) 7.6 us
+// with the weights in the memory-side cache, 9.0 us without; 777 x 513 over 784 13.5 us.  (Loads a step further ahead, with the
+// registers for it taken from the addresses, were slower: 14.5 us.)
 template <bool KC>
 __device__ __forceinline__ void direct_fragment(const float* __restrict__ p, int64_t ld, int64_t row, int64_t k, int64_t ke, bool vec,
                                                 float (&x)[8]) {

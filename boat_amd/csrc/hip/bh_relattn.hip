@@ -403,7 +403,7 @@ template <int DP> struct ForwardLds {
 
 // A workgroup owns 128 queries of a head, a wavefront 32 of them, and walks over the keys.  Keys and values have a place in
 // LDS each: the next keys are on their way while the values are worked on and the other way round.  Bound by the matrix cores and
-// the exponentials and splits beside them: 128 heads of 1024 x 1024 at head size 64 180 us, 190 TFLOP/s of fp32 products (a large
+// the exponentials and splits beside them (matrix cores busy for 61 % of the cycles): 128 heads of 1024 x 1024 at head size 64 180 us, 190 TFLOP/s of fp32 products (a large
 // library product in bf16 has 195 to offer at six products each), causal 121 us.
 template <int DP>
 __global__ __launch_bounds__(kThreads, 2) void relattn_forward_kernel(RelArgs g) {
@@ -479,7 +479,8 @@ __global__ __launch_bounds__(kThreads, 2) void relattn_forward_kernel(RelArgs g)
 }
 
 // ---- few query rows (of all the heads that share a key head together) over many keys: wavefronts split the keys, each reads
-// its keys and values once, straight into fragments.  One query of 64 heads over 8001 keys: 48 us, 5.4 TB/s.
+// its keys and values once, straight into fragments.  One query of 64 heads over 8001 keys (262 MB), with joining: 57 us where
+// the memory-side cache holds what it can of them from the call before, 67 us (3.9 TB/s) where it holds nothing.
 constexpr int kRowWaves = 4;
 template <int DP>
 __global__ __launch_bounds__(64 * kRowWaves, DP <= 96 ? 2 : 1) void relattn_rows_kernel(RelArgs g, int row_tiles) {
@@ -489,7 +490,8 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 96 ? 2 : 1) void relattn_rows
     __shared__ float part[kRowWaves][32][33];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // Each sequence's own keys are cut evenly, and the sequences take turns from part to part: the workgroups that share a compute
-    // unit (half a launch apart) then belong to a long and a short one (16 heads, lengths 8001, 5490, 4569, 5989: 47 us against 52).
+    // unit (half a launch apart) then belong to a long and a short one (16 heads, lengths 8001, 5490, 4569, 5989, one
+    // call after the other, 47 us against 52).
     const int rt = blockIdx.x % row_tiles, bk = blockIdx.x / row_tiles, hk = bk % g.kv_heads;
     const int bt = (bk / g.kv_heads + (int)((int64_t)blockIdx.y * g.batch / g.splits)) % g.batch;
     const int rows = g.group * (int)g.sq, r = min(32 * rt + (lane & 31), rows - 1);
@@ -1010,8 +1012,8 @@ __device__ __forceinline__ void key_tile(const RelArgs& g, int id, int part) {
 
 // Both walks in one launch: the key tiles, which take longer, first, and the query tiles fill up behind them (one launch after the
 // other, us: 128 heads of 1024, causal, 482 against 459; 32 heads of 1024 at head size 128 379 against 261).  Bound by the matrix
-// cores at seven products of a head's size (scores and dP are made in both walks: adding up dQ over the key tiles instead would
-// write and read it once per tile): 128 heads of 1024, causal, 410 us, 147 TFLOP/s.
+// cores (49 % of the cycles) at seven products of a head's size, as scores and dP are made in both walks: 128 heads of 1024, causal,
+// 420 us, 143 TFLOP/s.  Five products would do, with a part of dQ written for every key tile and the parts added up in order.
 template <int DP>
 __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void relattn_backward_kernel(RelArgs g, int key_groups, int query_groups) {
     const int all_keys = key_groups * g.q_splits, id = blockIdx.x;

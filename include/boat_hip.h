@@ -10,7 +10,8 @@
  *
  * The fused training operators (bh_gemm_epilogue, bh_dense_act_backward, bh_distill_*, bh_relbias_attention_*) take work
  * memory for the length of the call: several threads may call them, a stream capture in progress is refused (BH_EINVAL).
- * They take device pointers of any allocator; what another stream writes has to be finished before the call.
+ * They take device pointers of any allocator; what another stream writes has to be finished before the call, and the memory has to
+ * stay theirs until the library's stream is done with it (an allocator that orders reuse by its own streams does not know of it).
  *
  * Each kernel entry point names the reference routine (file:line under the Boat tree)
  * whose arithmetic it replaces.
@@ -283,14 +284,16 @@ int bh_dense_backward_into(const float* x, const float* w, const float* dy,
  * (C += act(z)); otherwise no output may overlap an operand.  K == 0: z = bias.
  * GELU is off by less than 2e-7 |z| and may differ in its last bits from bh_activation_forward's.
  * fp32 sums on the bf16 matrix cores (each operand as the exact sum of three bf16, six partial products: the error of an
- * fp32 product and sum); infinities and NaN come out as fp32 arithmetic gives them.  An infinite sum is made again term by term:
- * a matrix full of them takes up to 200 times as long as a finite one, a matrix of NaN about twice as long. */
+ * fp32 product and sum); infinities and NaN come out as fp32 arithmetic gives them.  An infinite sum, and one with a
+ * value past the largest bf16 (3.39e38), is made again term by term: a matrix full of them takes up to 200 times as long as
+ * another, a matrix of NaN about twice as long. */
 int bh_gemm_epilogue(int trans_a, int trans_b, int64_t m, int64_t n, int64_t k, const float* a, int64_t lda, const float* b,
                      int64_t ldb, float* c, int64_t ldc, const float* bias, int act, float* saved, int64_t lds,
                      const float* residual, int64_t ldr);
 /* Backward of y[m,n] = act(x[m,k] . w[k,n] + b) + residual, all dense: dz = dy * act'(saved); dx = dz . w^T (assigned),
  * gw = x^T . dz and gb = column sums of dz (assigned, or added with accumulate != 0).  Any of dx, gw, gb may be NULL.  The
- * residual's gradient is dy itself.  saved: as bh_gemm_epilogue left it (not read for BH_ACT_NONE). */
+ * residual's gradient is dy itself.  saved: as bh_gemm_epilogue left it (not read for BH_ACT_NONE).  No output may overlap an
+ * operand. */
 int bh_dense_act_backward(int act, const float* x, const float* w, const float* saved, const float* dy, float* dx, float* gw,
                           float* gb, int64_t m, int64_t k, int64_t n, int accumulate);
 
@@ -347,7 +350,7 @@ int bh_relbias_attention_forward(const bh_relbias_attention_t* p, const float* q
                                  const float* table, const int32_t* kv_len, float* out, float* lse);
 /* out and lse: of the forward call.  d_out has the strides of out; dq, dk, dv those of q, k, v (assigned; zero at keys behind
  * kv_len; the heads that share a key head add up); dtable [num_buckets, heads] is assigned, or added to with
- * accumulate_table != 0.  The same inputs give the same bits every time. */
+ * accumulate_table != 0.  The same inputs give the same bits every time.  No output of either call may overlap an operand. */
 int bh_relbias_attention_backward(const bh_relbias_attention_t* p, const float* q, const float* k, const float* v,
                                   const float* table, const int32_t* kv_len, const float* out, const float* lse,
                                   const float* d_out, float* dq, float* dk, float* dv, float* dtable, int accumulate_table);
