@@ -16,6 +16,7 @@
 // written over the dense ones behind a barrier.
 #include "bh_common.h"
 
+#include <float.h>
 #include <math.h>
 
 #include <type_traits>
@@ -462,8 +463,9 @@ static int distill_check(const char* fn, const float* z, int64_t ldz, const floa
     if (vocab > (1 << 30) || rows > (1 << 22)) return set_error(BH_EINVAL, "%s: too many rows or too large a vocabulary", fn);
     if (topk > kMaxTopk) return set_error(BH_EINVAL, "%s: topk is at most %d", fn, kMaxTopk);
     if (ldz < vocab) return set_error(BH_EINVAL, "%s: leading dimension too small", fn);
-    // T^2 weighs the loss and 1/T the logits: both have to be numbers
-    if (!(temperature > 0.f) || !(temperature * temperature < INFINITY) || !(kLog2e / temperature < INFINITY))
+    // T^2 weighs the loss and 1/T the logits: both have to be numbers (a square of 0 would make NaN of a large divergence)
+    if (!(temperature > 0.f) || !(temperature * temperature >= FLT_MIN) || !(temperature * temperature < INFINITY) ||
+        !(kLog2e / temperature < INFINITY))
         return set_error(BH_EINVAL, "%s: the temperature is a positive number whose square and inverse are in range", fn);
     if (!(alpha >= 0.f && alpha <= 1.f)) return set_error(BH_EINVAL, "%s: alpha lies in [0, 1]", fn);
     if (rows > 0 && (!z || (topk > 0 && (!teacher || !index)))) return set_error(BH_EINVAL, "%s: null pointer", fn);

@@ -179,11 +179,11 @@ int bh_softmax_ce_grad(const float* logits, const int32_t* labels, float* dlogit
  * row without any, or with logits of -inf only, has no teacher part), q = softmax(logits / T) and r = softmax(logits):
  *   row_loss = alpha T^2 sum_j p_j (log p_j - log q[index_j]) + (1 - alpha) (-log r[label]),   loss_out[0] = scale * sum of row_loss
  *   dlogits  = seed * scale * (alpha T (q - p) + (1 - alpha) (r - onehot(label)))
- * Without labels the second term is absent, with alpha = 0 the first (the teacher is not read).  0 <= topk <= 4096, T > 0,
- * alpha in [0, 1], at most 2^22 rows and 2^30 entries of the vocabulary.  row_loss [rows], stats [3 * rows] and loss_out [1] may
- * be NULL.  bh_distill_backward takes the stats of a forward call on the same arguments and seed (one float in device memory,
- * NULL = 1); bh_distill_loss_grad is both passes in one (seed 1), reading the logits once.  Masked logits may be -inf or any
- * large negative number; a row of -inf only, +inf and NaN make their row NaN.
+ * Without labels the second term is absent, with alpha = 0 the first (the teacher is not read).  0 <= topk <= 4096, T > 0 (its
+ * square in range), alpha in [0, 1], at most 2^22 rows and 2^30 entries of the vocabulary.  row_loss [rows], stats [3 * rows] and
+ * loss_out [1] may be NULL.  bh_distill_backward takes the stats of a forward call on the same arguments and seed (one float in
+ * device memory, NULL = 1); bh_distill_loss_grad is both passes in one (seed 1), reading the logits once.  Masked logits may be
+ * -inf or any large negative number; a row of -inf only, and one with +inf or NaN, is NaN, loss and gradient, and no other is.
  * dlogits may be logits itself (ldd == ld); no other overlap. */
 int bh_distill_forward(const float* logits, int64_t ld, const float* teacher, const int32_t* index, const int32_t* labels,
                        int64_t rows, int64_t vocab, int64_t topk, float temperature, float alpha, float scale,

@@ -102,3 +102,24 @@ def test_on_the_tape(boat, rng):
     for t in [eager, *made]:
         boat.boat_tensor_unref(t)
     assert not boat.boat_has_error()
+
+
+@pytest.mark.parametrize("rows", [0, 1])
+def test_keys_that_all_sequences_share(hip, rng, rows):
+    """A stride of zero over the batch (one prompt for all) or over the key heads, read but never written."""
+    q, k, v, table, _ = attention_case(rng, 3, 4, 2, 20, 150, 48, 16)
+    for axis in (0, 1):
+        one = [np.ascontiguousarray(np.take(x, [0], axis)) for x in (k, v)]
+        ks = [one[0].shape[1] * 150 * 48, 150 * 48, 48]
+        ks[axis] = 0
+        plan = hip.relbias_attention(batch=3, heads=4, kv_heads=2, sq=20, sk=150, d=48, q_stride=(4 * 20 * 48, 20 * 48, 48), k_stride=ks, v_stride=ks,
+                                     o_stride=(4 * 20 * 48, 20 * 48, 48), query_offset=130, num_buckets=16, max_distance=60, bidirectional=0, causal=1,
+                                     scale=0.125)
+        out, lse = dev(hip, np.full(q.shape, np.nan, np.float32)), dev(hip, np.full(q.shape[:3], np.nan, np.float32))
+        hip.check(hip.bh_relbias_attention_force_rows(rows))
+        try:
+            hip.check(hip.bh_relbias_attention_forward(plan, ptr(dev(hip, q)), *(ptr(dev(hip, x)) for x in one), ptr(dev(hip, table)), None, ptr(out), ptr(lse)))
+        finally:
+            hip.check(hip.bh_relbias_attention_force_rows(-1))
+        want, bound = oc.attention(q, *(np.repeat(x, k.shape[axis], axis) for x in one), table, None, 130, 16, 60, False, True, 0.125)
+        assert (np.abs(out.numpy() - want["out"]) <= bound["out"]).all() and (np.abs(lse.numpy() - want["lse"]) <= bound["lse"]).all()

@@ -125,3 +125,33 @@ def test_a_teacher_without_weight_is_not_looked_at(hip, rng, rows, vocab):
         got = run_distill(hip, z, t, index, lab, 2.0, 0.0, 0.5)
         assert np.array_equal(got[0][0], want[0][0]) and got[0][1] == want[0][1] and np.array_equal(got[1][0], want[1][0])
         assert np.array_equal(got[2], want[2]) and np.array_equal(got[3], want[3])
+
+
+@pytest.mark.parametrize("rows,vocab", SHAPES)
+@pytest.mark.parametrize("temperature", [1.0, 2.5])
+def test_rows_without_a_softmax(hip, rng, rows, vocab, temperature):
+    """-inf all over a row, +inf or NaN in it: that row is NaN, the others are what they are without it."""
+    z, teacher, index, lab = distill_case(rng, rows, vocab, 6)
+    index[0], lab[0] = 0, 0                                      # the spoilt row has entries and a label
+    want = run_distill(hip, z, teacher, index, lab, temperature, 0.5, 0.5)
+    for spoil in ("empty", np.inf, np.nan):
+        bad = z.copy()
+        if spoil == "empty":
+            bad[0] = -np.inf
+        else:
+            bad[0, vocab // 2] = spoil
+        (row, loss), (row2, loss2), dz, back = run_distill(hip, bad, teacher, index, lab, temperature, 0.5, 0.5)
+        assert np.isnan([row[0], row2[0], loss, loss2]).all() and np.isnan(dz[0]).all() and np.isnan(back[0]).all(), spoil
+        assert np.array_equal(row[1:], want[0][0][1:]) and np.array_equal(row2[1:], want[1][0][1:])
+        assert np.array_equal(dz[1:], want[2][1:]) and np.array_equal(back[1:], want[3][1:])
+
+
+def test_more_rows_than_a_grids_second_dimension(hip, rng):
+    rows, vocab = 66000, 33
+    z, teacher, index, lab = distill_case(rng, rows, vocab, 3)
+    want_row, want_loss, want_dz = oc.distill(z, teacher, index, lab, 2.0, 0.5, 1.0 / rows)
+    tol_row, tol_dz = bounds(z, teacher, 2.0, 0.5, 1.0 / rows, vocab)
+    (row, loss), (row2, _), dz, back = run_distill(hip, z, teacher, index, lab, 2.0, 0.5, 1.0 / rows)
+    assert (np.abs(row - want_row) <= tol_row + 4 * oc.U * np.abs(want_row)).all() and np.array_equal(row, row2)
+    assert abs(loss - want_loss) <= tol_row + 4 * oc.U * abs(want_loss)
+    assert (np.abs(dz - want_dz) <= tol_dz).all() and (np.abs(back - 2 * want_dz) <= 2 * tol_dz).all()
